@@ -1,0 +1,702 @@
+// Attention over packed sequences of different lengths: causal or not, grouped heads, head dims up to
+// 128, bf16 and fp32, forward and backward (reference core: manifold_layers.py:404-427).
+//
+// Rows.  The G = hq / hkv query heads that share a key / value head are packed into the rows of one
+// tile: packed row r of a sequence is (token r / G, head r % G), so a key / value tile is read once for
+// the whole group and the gradient of a shared head is summed in registers.
+//
+// Orientation.  Scores are formed transposed, S^T = K Q^T, with 32x32 matrix tiles: a lane then holds
+// 16 scores of ONE query (column lane & 31; keys 8 (r / 4) + 4 (lane >> 5) + r % 4 for register r), so a
+// softmax row is 16 registers and one exchange between the two lane halves, and the running maximum and
+// sums are one register each.  The contraction index of the second product may be numbered freely: with
+// key slot (h, e) = key 16 s + 8 (e / 4) + 4 h + e % 4 the accumulator registers 8 s .. 8 s + 7 ARE the
+// second operand of O^T += V^T P^T (no lane exchange), and V is read from LDS with the transposing load.
+// The backward uses the same two moves for dQ^T += K^T dS^T, dV^T += dO^T P and dK^T += Q^T dS.
+//
+// LDS tiles are rows of DP elements (DP = d rounded up to 32 / 64 / 128, columns >= d zero) whose 16-byte
+// chunks are permuted by a function of the row, so that both the row reads (8 rows of one chunk) and the
+// transposing reads (4 rows of two chunks) touch every bank once.
+#include "hv_common.h"
+
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int NT = 256;         // threads of every block: 4 waves
+constexpr float NEG_INF = -__builtin_inff();
+
+template <typename T> struct Frag;                       // 8 values of a lane: one operand over 16 columns
+template <> struct Frag<unsigned short> { bf16x8 v; };
+template <> struct Frag<float> { float v[8]; };
+
+__device__ __forceinline__ f32x16 mma16(const Frag<unsigned short>& a, const Frag<unsigned short>& b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, b.v, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma16(const Frag<float>& a, const Frag<float>& b, f32x16 c) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[e], b.v[e], c, 0, 0, 0);
+  return c;
+}
+
+template <typename T, int DP> struct Lay {               // an LDS tile
+  static constexpr int ROWB = DP * (int)sizeof(T);       // bytes of a row
+  static constexpr int CH = ROWB / 16;                   // its 16-byte chunks
+  static constexpr int EPC = 16 / (int)sizeof(T);        // elements of a chunk
+  static constexpr int NS = DP / 16, NDT = DP / 32;      // 16-column steps, 32-column tiles
+  static __device__ __forceinline__ int f(int row) {     // chunk permutation of a row (rows = 0 mod 8: 0)
+    return CH >= 8 ? ((row & 3) << 1) | ((row >> 2) & 1) : (row & 2) | ((row >> 2) & 1);
+  }
+};
+
+// a wave's view of a tile: lane constants of the two kinds of operand reads
+template <typename T, int DP> struct View {
+  using L = Lay<T, DP>;
+  int row_base, row_x, tr_base, tr_x;
+  __device__ __forceinline__ View(int lane) {
+    const int h = lane >> 5, m = lane & 31;
+    row_base = m * L::ROWB;
+    if constexpr (sizeof(T) == 2) {
+      row_x = (h ^ L::f(m)) << 4;
+      const int i = lane & 15, rl = 4 * h + (i >> 2);
+      tr_base = rl * L::ROWB + (i & 1) * 8;
+      tr_x = ((2 * ((lane >> 4) & 1) + ((i >> 1) & 1)) ^ L::f(rl)) << 4;
+    } else {
+      row_x = ((2 * h) ^ L::f(m)) << 4;
+      tr_base = 4 * h * L::ROWB + (m & 3) * 4;
+      tr_x = ((m >> 2) ^ h) << 4;                        // f(4 h + e) = 2 e | h; the 2 e part is added per element
+    }
+  }
+  // operand over columns 16 s .. 16 s + 15 of the 32 rows from `tile` (a multiple of 32 rows into the tile)
+  __device__ __forceinline__ Frag<T> rows(const char* tile, int s) const {
+    Frag<T> r;
+    if constexpr (sizeof(T) == 2) {
+      r.v = *(const bf16x8*)(tile + row_base + (row_x ^ (s << 5)));
+    } else {
+      const f32x4 a = *(const f32x4*)(tile + row_base + (row_x ^ (s << 6)));
+      const f32x4 b = *(const f32x4*)(tile + row_base + (row_x ^ (s << 6) ^ 16));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { r.v[e] = a[e]; r.v[4 + e] = b[e]; }
+    }
+    return r;
+  }
+  // transposed operand: columns 32 dt .. 32 dt + 31 as rows, the 16 tile rows from `tile` (a multiple of 8 rows
+  // into the tile) as contraction slots
+  __device__ __forceinline__ Frag<T> cols(const char* tile, int dt) const {
+    Frag<T> r;
+    if constexpr (sizeof(T) == 2) {
+      typedef __attribute__((address_space(3))) s16x4 lds4;
+      const char* p = tile + tr_base + (tr_x ^ (dt << 6));
+      union { s16x4 q[2]; bf16x8 v; } u;
+      u.q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p));
+      u.q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 8 * L::ROWB));
+      r.v = u.v;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        r.v[e] = *(const float*)(tile + (8 * (e >> 2) + (e & 3)) * L::ROWB + tr_base +
+                                 (tr_x ^ (dt << 7) ^ ((e & 3) << 5)));
+    }
+    return r;
+  }
+};
+
+// accumulator registers 8 s .. 8 s + 7 as the second operand of the next product
+template <typename T> __device__ __forceinline__ Frag<T> from_acc(const f32x16& c, int s) {
+  Frag<T> r;
+  if constexpr (sizeof(T) == 2) {
+    u32x4 u;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) u[e] = pack_bf16x2(c[8 * s + 2 * e], c[8 * s + 2 * e + 1]);
+    r.v = __builtin_bit_cast(bf16x8, u);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r.v[e] = c[8 * s + e];
+  }
+  return r;
+}
+
+// sum of the 8 values as the product sees them (rounded to T), added to c
+__device__ __forceinline__ float add_sum(const Frag<unsigned short>& p, float c) {
+  const u32x4 u = __builtin_bit_cast(u32x4, p.v);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    c += __uint_as_float(u[e] << 16) + __uint_as_float(u[e] & 0xffff0000u);
+  return c;
+}
+__device__ __forceinline__ float add_sum(const Frag<float>& p, float c) {
+  return c + (((p.v[0] + p.v[1]) + (p.v[2] + p.v[3])) + ((p.v[4] + p.v[5]) + (p.v[6] + p.v[7])));
+}
+
+__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
+
+// ------------------------------------------------------------------------------------------------
+// Which rows a block works on: the sequences (and the rows before the first and behind the last one, two
+// more "sequences" without keys) cut into tiles of BM packed rows, numbered through.  Every wave scans the
+// offsets by itself, 64 sequences at a time.
+struct Tile { int seq, start, len, tile; };              // seq -1: no such tile; start, len: its rows in tokens
+
+__device__ __forceinline__ int clamp_row(int v, int total) { return v < 0 ? 0 : (v > total ? total : v); }
+
+__device__ __forceinline__ Tile find_tile(const int* __restrict__ cu, int nseq, long total_l, int G, int BM, int idx,
+                                          bool reverse) {
+  const int lane = threadIdx.x & 63, total = (int)total_l;
+  Tile t{-1, 0, 0, 0};
+  int before = 0;
+  for (int s0 = 0; s0 < nseq + 2; s0 += 64) {
+    const int s = s0 + lane;
+    int a = 0, b = 0;
+    if (s < nseq) {
+      a = clamp_row(cu[s], total);
+      b = clamp_row(cu[s + 1], total);
+    } else if (s == nseq) {
+      b = clamp_row(cu[0], total);
+    } else if (s == nseq + 1) {
+      a = clamp_row(cu[nseq], total);
+      b = total;
+    }
+    if (b < a) b = a;
+    const int n = (int)(((long)(b - a) * G + BM - 1) / BM);
+    int upto = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int v = __shfl_up(upto, o, 64);
+      if (lane >= o) upto += v;
+    }
+    const unsigned long long hit = __ballot(idx < before + upto);
+    if (hit) {
+      const int src = __builtin_ctzll(hit);
+      t.seq = s0 + src;
+      t.start = __builtin_amdgcn_readlane(a, src);
+      t.len = __builtin_amdgcn_readlane(b, src) - t.start;
+      const int nt = __builtin_amdgcn_readlane(n, src);
+      t.tile = idx - before - (__builtin_amdgcn_readlane(upto, src) - nt);
+      if (reverse) t.tile = nt - 1 - t.tile;
+      return t;
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+  return t;
+}
+
+// rows of sequence `seq` on the other side (none for the two outside ranges)
+__device__ __forceinline__ void seq_rows(const int* __restrict__ cu, int nseq, long total, int seq, int& start, int& len) {
+  if (seq >= nseq) { start = len = 0; return; }
+  start = clamp_row(cu[seq], (int)total);
+  len = clamp_row(cu[seq + 1], (int)total) - start;
+  if (len < 0) len = 0;
+}
+
+// 16-byte chunks of ROWS tile rows -> registers -> LDS; source row `row` of the tile is src(row)'s address or
+// null (zeros), chunks at columns >= d are zero
+template <typename T, int DP, int ROWS> struct Stage {
+  using L = Lay<T, DP>;
+  static constexpr int N = ROWS * L::CH / NT;
+  static_assert(N * NT == ROWS * L::CH, "whole chunks per thread");
+  u32x4 r[N];
+  template <typename F> __device__ __forceinline__ void load(int d, F src) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int i = threadIdx.x + n * NT, row = i / L::CH, c = i % L::CH;
+      const T* p = src(row);
+      r[n] = (p != nullptr && c * L::EPC < d) ? *(const u32x4*)(p + c * L::EPC) : u32x4{0, 0, 0, 0};
+    }
+  }
+  __device__ __forceinline__ void store(char* tile) const {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int i = threadIdx.x + n * NT, row = i / L::CH, c = i % L::CH;
+      *(u32x4*)(tile + row * L::ROWB + ((c ^ L::f(row)) << 4)) = r[n];
+    }
+  }
+};
+
+// a lane's row of 16-column operands straight from memory (null: zeros)
+template <typename T, int DP> __device__ __forceinline__ void load_row(Frag<T>* f, const T* p, int d, int h) {
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) {
+    const int c = 16 * s + 8 * h;
+    const bool in = p != nullptr && c < d;
+    if constexpr (sizeof(T) == 2) {
+      f[s].v = in ? *(const bf16x8*)(p + c) : bf16x8{};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) {
+        const f32x4 a = in ? *(const f32x4*)(p + c + e) : f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) f[s].v[e + x] = a[x];
+      }
+    }
+  }
+}
+
+// four consecutive values of a lane's row
+__device__ __forceinline__ void store4(unsigned short* p, float a, float b, float c, float d) {
+  *(uint2*)p = make_uint2(pack_bf16x2(a, b), pack_bf16x2(c, d));
+}
+__device__ __forceinline__ void store4(float* p, float a, float b, float c, float d) {
+  *(float4*)p = make_float4(a, b, c, d);
+}
+
+template <typename T, int DP>
+__device__ __forceinline__ void store_row(T* p, int d, int h, const f32x16* acc, float mul) {
+#pragma unroll
+  for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int c = 32 * dt + 8 * g + 4 * h;
+      if (c < d)
+        store4(p + c, acc[dt][4 * g] * mul, acc[dt][4 * g + 1] * mul, acc[dt][4 * g + 2] * mul, acc[dt][4 * g + 3] * mul);
+    }
+}
+
+__device__ __forceinline__ f32x16 zero16() {
+  f32x16 z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.f;
+  return z;
+}
+
+// ------------------------------------------------------------------------------------------------
+// Forward: 4 waves of 32 packed rows each over tiles of BN keys that the block stages once.
+template <typename T, int DP, bool TRAIN>
+__global__ void __launch_bounds__(NT) k_attn_packed(const hv_attn_packed_args a) {
+  using L = Lay<T, DP>;
+  constexpr int BM = 128, BN = 64, TB = BN * L::ROWB;
+  __shared__ __align__(16) char smem[2 * TB];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  const int kvh = blockIdx.x % a.hkv, G = a.hq / a.hkv;
+  const Tile t = find_tile(a.cu_q, a.nseq, a.total_q, G, BM, blockIdx.x / a.hkv, a.causal != 0);
+  if (t.seq < 0) return;
+  int k0, lk;
+  seq_rows(a.cu_k, a.nseq, a.total_k, t.seq, k0, lk);
+
+  const long r = (long)t.tile * BM + wave * 32 + (lane & 31);
+  const bool real = r < (long)t.len * G;
+  const int tok = real ? (int)(r / G) : 0, g = (int)(r % G);
+  const int late = lk - t.len;                           // the last query sees every key
+  const int lim = !real ? -1 : (a.causal ? min(tok + late, lk - 1) : lk - 1);     // last key of this row
+  // the block's last key, the wave's first row's last key: full tiles need no mask
+  const long last_r = min((long)(t.tile + 1) * BM, (long)t.len * G) - 1;
+  const int lim_blk = a.causal ? min((int)(last_r / G) + late, lk - 1) : lk - 1;
+  int lim_lo = lim, lim_hi = lim;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    lim_lo = min(lim_lo, __shfl_xor(lim_lo, o, 64));
+    lim_hi = max(lim_hi, __shfl_xor(lim_hi, o, 64));
+  }
+  lim_lo = __builtin_amdgcn_readfirstlane(lim_lo);
+  lim_hi = __builtin_amdgcn_readfirstlane(lim_hi);
+
+  const long qrow = (long)t.start + tok;
+  const int qh = kvh * G + g;
+  Frag<T> q[L::NS];
+  load_row<T, DP>(q, real ? (const T*)a.q + qrow * a.q_row + (long)qh * a.q_head : nullptr, a.d, h);
+  const T* kp = (const T*)a.k + (long)k0 * a.k_row + (long)kvh * a.k_head;
+  const T* vp = (const T*)a.v + (long)k0 * a.v_row + (long)kvh * a.v_head;
+
+  f32x16 o[L::NDT];
+#pragma unroll
+  for (int i = 0; i < L::NDT; ++i) o[i] = zero16();
+  float m = NEG_INF, l = 0.f, lt = 0.f;                  // running maximum, sum of rounded / of exact weights
+  const float c2 = a.scale * LOG2E;
+  const View<T, DP> view(lane);
+  const int ntile = (lim_blk + BN) / BN;
+
+  Stage<T, DP, BN> sk, sv;
+  auto fetch = [&](int kt) {
+    sk.load(a.d, [&](int row) { const int j = kt * BN + row; return j <= lim_blk ? kp + (long)j * a.k_row : nullptr; });
+    sv.load(a.d, [&](int row) { const int j = kt * BN + row; return j <= lim_blk ? vp + (long)j * a.v_row : nullptr; });
+  };
+  if (ntile > 0) fetch(0);
+  for (int kt = 0; kt < ntile; ++kt) {
+    __syncthreads();
+    sk.store(smem);
+    sv.store(smem + TB);
+    __syncthreads();
+    if (kt + 1 < ntile) fetch(kt + 1);
+    if (kt * BN > lim_hi) continue;
+    f32x16 s[2] = {zero16(), zero16()};
+#pragma unroll
+    for (int i = 0; i < L::NS; ++i) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) s[j] = mma16(view.rows(smem + j * 32 * L::ROWB, i), q[i], s[j]);
+    }
+    if (kt * BN + BN - 1 > lim_lo) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int x = 0; x < 16; ++x)
+          if (kt * BN + 32 * j + 8 * (x >> 2) + 4 * h + (x & 3) > lim) s[j][x] = NEG_INF;
+    }
+    float top = s[0][0];
+#pragma unroll
+    for (int x = 1; x < 16; ++x) top = fmaxf(top, s[0][x]);
+#pragma unroll
+    for (int x = 0; x < 16; ++x) top = fmaxf(top, s[1][x]);
+    top = fmaxf(top, other_half(top));
+    // the running maximum moves only when a score passes it by 8 powers of two: weights stay below 2^8 and
+    // the accumulators are seldom rescaled
+    if (__any((top - m) * c2 > 8.f)) {
+      const float mn = fmaxf(m, top);
+      const float alpha = mn == NEG_INF ? 1.f : __builtin_amdgcn_exp2f((m - mn) * c2);
+      m = mn;
+      l *= alpha;
+      lt *= alpha;
+#pragma unroll
+      for (int i = 0; i < L::NDT; ++i)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) o[i][x] *= alpha;
+    }
+    const float mc = m == NEG_INF ? 0.f : -m * c2;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) s[j][x] = __builtin_amdgcn_exp2f(fmaf(s[j][x], c2, mc));
+    if constexpr (TRAIN && sizeof(T) == 2) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) lt += s[j][x];
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const Frag<T> p = from_acc<T>(s[j], i);
+        l = add_sum(p, l);
+#pragma unroll
+        for (int dt = 0; dt < L::NDT; ++dt)
+          o[dt] = mma16(view.cols(smem + TB + (32 * j + 16 * i) * L::ROWB, dt), p, o[dt]);
+      }
+  }
+  if (!real) return;
+  l += other_half(l);
+  if constexpr (TRAIN && sizeof(T) == 2) lt += other_half(lt); else lt = l;
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+  const long orow = (qrow * a.hq + qh) * a.d;
+  store_row<T, DP>((T*)a.out + orow, a.d, h, o, inv);
+  if constexpr (TRAIN) {
+    if (h == 0 && a.lse) a.lse[qrow * a.hq + qh] = lt > 0.f || lt != lt ? m * a.scale + __logf(lt) : NEG_INF;
+    if constexpr (sizeof(T) == 2) {
+      if (a.out_low) {
+#pragma unroll
+        for (int dt = 0; dt < L::NDT; ++dt)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) {
+            const float v = o[dt][x] * inv;
+            o[dt][x] = v - bf2f(f2bf(v));
+          }
+        store_row<T, DP>((T*)a.out_low + orow, a.d, h, o, 1.f);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// delta_i = dO_i . O_i = sum_j P_ij dP_ij (the mean that the softmax gradient subtracts): one wave per row
+template <typename T>
+__global__ void __launch_bounds__(NT) k_attn_packed_delta(const hv_attn_packed_args a, float* __restrict__ delta) {
+  const int lane = threadIdx.x & 63;
+  for (long i = (long)blockIdx.x * 4 + (threadIdx.x >> 6); i < a.total_q * a.hq; i += (long)gridDim.x * 4) {
+    const long row = i / a.hq;
+    const T* po = (const T*)a.out + i * a.d;
+    const T* pl = (const T*)a.out_low;
+    const T* pd = (const T*)a.dout + row * a.do_row + (i % a.hq) * a.do_head;
+    float s = 0.f;
+    for (int c = lane; c < a.d; c += 64) {
+      float v = Elem<T>::load(po, c);
+      if (pl) v += Elem<T>::load(pl + i * a.d, c);
+      s = fmaf(v, Elem<T>::load(pd, c), s);
+    }
+    s = wave_sum(s);
+    if (lane == 0) delta[i] = s;
+  }
+}
+
+// dQ: the forward's walk over the keys with dO beside Q; dQ^T += K^T dS^T
+template <typename T, int DP>
+__global__ void __launch_bounds__(NT) k_attn_packed_dq(const hv_attn_packed_args a, const float* __restrict__ delta) {
+  using L = Lay<T, DP>;
+  constexpr int BM = 128, BN = 64, TB = BN * L::ROWB;
+  __shared__ __align__(16) char smem[2 * TB];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  const int kvh = blockIdx.x % a.hkv, G = a.hq / a.hkv;
+  const Tile t = find_tile(a.cu_q, a.nseq, a.total_q, G, BM, blockIdx.x / a.hkv, a.causal != 0);
+  if (t.seq < 0) return;
+  int k0, lk;
+  seq_rows(a.cu_k, a.nseq, a.total_k, t.seq, k0, lk);
+  const long r = (long)t.tile * BM + wave * 32 + (lane & 31);
+  const bool real = r < (long)t.len * G;
+  const int tok = real ? (int)(r / G) : 0, g = (int)(r % G);
+  const int late = lk - t.len;
+  const int lim = !real ? -1 : (a.causal ? min(tok + late, lk - 1) : lk - 1);
+  const long last_r = min((long)(t.tile + 1) * BM, (long)t.len * G) - 1;
+  const int lim_blk = a.causal ? min((int)(last_r / G) + late, lk - 1) : lk - 1;
+  int lim_lo = lim, lim_hi = lim;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    lim_lo = min(lim_lo, __shfl_xor(lim_lo, o, 64));
+    lim_hi = max(lim_hi, __shfl_xor(lim_hi, o, 64));
+  }
+  lim_lo = __builtin_amdgcn_readfirstlane(lim_lo);
+  lim_hi = __builtin_amdgcn_readfirstlane(lim_hi);
+  const long qrow = (long)t.start + tok;
+  const int qh = kvh * G + g;
+  Frag<T> q[L::NS], go[L::NS];
+  load_row<T, DP>(q, real ? (const T*)a.q + qrow * a.q_row + (long)qh * a.q_head : nullptr, a.d, h);
+  load_row<T, DP>(go, real ? (const T*)a.dout + qrow * a.do_row + (long)qh * a.do_head : nullptr, a.d, h);
+  const float c2 = a.scale * LOG2E;
+  float le = real ? a.lse[qrow * a.hq + qh] : 0.f;
+  le = le == NEG_INF ? 0.f : -le * LOG2E;
+  const float dl = real ? delta[qrow * a.hq + qh] : 0.f;
+  const T* kp = (const T*)a.k + (long)k0 * a.k_row + (long)kvh * a.k_head;
+  const T* vp = (const T*)a.v + (long)k0 * a.v_row + (long)kvh * a.v_head;
+
+  f32x16 dq[L::NDT];
+#pragma unroll
+  for (int i = 0; i < L::NDT; ++i) dq[i] = zero16();
+  const View<T, DP> view(lane);
+  const int ntile = (lim_blk + BN) / BN;
+  Stage<T, DP, BN> sk, sv;
+  auto fetch = [&](int kt) {
+    sk.load(a.d, [&](int row) { const int j = kt * BN + row; return j <= lim_blk ? kp + (long)j * a.k_row : nullptr; });
+    sv.load(a.d, [&](int row) { const int j = kt * BN + row; return j <= lim_blk ? vp + (long)j * a.v_row : nullptr; });
+  };
+  if (ntile > 0) fetch(0);
+  for (int kt = 0; kt < ntile; ++kt) {
+    __syncthreads();
+    sk.store(smem);
+    sv.store(smem + TB);
+    __syncthreads();
+    if (kt + 1 < ntile) fetch(kt + 1);
+#pragma unroll 1
+    for (int j = 0; j < 2; ++j) {
+      const int key = kt * BN + 32 * j;
+      if (key > lim_hi) break;
+      f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+      for (int i = 0; i < L::NS; ++i) {
+        s = mma16(view.rows(smem + j * 32 * L::ROWB, i), q[i], s);
+        dp = mma16(view.rows(smem + TB + j * 32 * L::ROWB, i), go[i], dp);
+      }
+      if (key + 31 > lim_lo) {
+#pragma unroll
+        for (int x = 0; x < 16; ++x)
+          if (key + 8 * (x >> 2) + 4 * h + (x & 3) > lim) s[x] = NEG_INF;
+      }
+#pragma unroll
+      for (int x = 0; x < 16; ++x) s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], c2, le)) * (dp[x] - dl);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const Frag<T> p = from_acc<T>(s, i);
+#pragma unroll
+        for (int dt = 0; dt < L::NDT; ++dt)
+          dq[dt] = mma16(view.cols(smem + (32 * j + 16 * i) * L::ROWB, dt), p, dq[dt]);
+      }
+    }
+  }
+  if (real) store_row<T, DP>((T*)a.dq + (qrow * a.hq + qh) * a.d, a.d, h, dq, a.scale);
+}
+
+// dK, dV: a wave holds 32 keys and walks over the packed rows of its sequence (all heads of the group)
+template <typename T, int DP>
+__global__ void __launch_bounds__(NT, 1) k_attn_packed_dkv(const hv_attn_packed_args a, const float* __restrict__ delta) {
+  using L = Lay<T, DP>;
+  constexpr int BK = 128, BR = L::ROWB >= 512 ? 32 : 64, TB = BR * L::ROWB;
+  __shared__ __align__(16) char smem[2 * TB];
+  __shared__ __align__(16) float st[2][BR];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+  const int kvh = blockIdx.x % a.hkv, G = a.hq / a.hkv;
+  const Tile t = find_tile(a.cu_k, a.nseq, a.total_k, 1, BK, blockIdx.x / a.hkv, false);
+  if (t.seq < 0) return;
+  int q0, lq;
+  seq_rows(a.cu_q, a.nseq, a.total_q, t.seq, q0, lq);
+  const int key = t.tile * BK + wave * 32 + (lane & 31);
+  const bool real = key < t.len;
+  const long krow = (long)t.start + key;
+  Frag<T> kf[L::NS], vf[L::NS];
+  load_row<T, DP>(kf, real ? (const T*)a.k + krow * a.k_row + (long)kvh * a.k_head : nullptr, a.d, h);
+  load_row<T, DP>(vf, real ? (const T*)a.v + krow * a.v_row + (long)kvh * a.v_head : nullptr, a.d, h);
+  const int late = t.len - lq;
+  // causal: row (token i) sees key j iff i >= j - late
+  const int first_tok = a.causal ? max(t.tile * BK - late, 0) : 0;
+  const int first_mine = a.causal ? key - late : 0;      // first token that sees this lane's key
+  const int wave_last = a.causal ? t.tile * BK + wave * 32 + 31 - late : 0;   // token that sees all of the wave's keys
+  const long rows = (long)lq * G;
+  const long r0 = (long)first_tok * G / BR * BR;
+  const float c2 = a.scale * LOG2E;
+
+  f32x16 dk[L::NDT], dv[L::NDT];
+#pragma unroll
+  for (int i = 0; i < L::NDT; ++i) { dk[i] = zero16(); dv[i] = zero16(); }
+  const View<T, DP> view(lane);
+  const T* qp = (const T*)a.q + (long)q0 * a.q_row + (long)kvh * G * a.q_head;
+  const T* gp = (const T*)a.dout + (long)q0 * a.do_row + (long)kvh * G * a.do_head;
+  const long sbase = (long)q0 * a.hq + (long)kvh * G;
+  Stage<T, DP, BR> sq, sg;
+  float stat = 0.f;
+  auto fetch = [&](long rr) {
+    sq.load(a.d, [&](int row) {
+      const long x = rr + row;
+      return x < rows ? qp + (x / G) * a.q_row + (x % G) * a.q_head : nullptr;
+    });
+    sg.load(a.d, [&](int row) {
+      const long x = rr + row;
+      return x < rows ? gp + (x / G) * a.do_row + (x % G) * a.do_head : nullptr;
+    });
+    if (threadIdx.x < 2 * BR) {
+      const long x = rr + (threadIdx.x & (BR - 1));
+      stat = 0.f;
+      if (x < rows) {
+        const long at = sbase + (x / G) * a.hq + x % G;
+        if (threadIdx.x < BR) {
+          const float le = a.lse[at];
+          stat = le == NEG_INF ? 0.f : -le * LOG2E;
+        } else {
+          stat = delta[at];
+        }
+      }
+    }
+  };
+  if (r0 < rows) fetch(r0);
+  for (long rr = r0; rr < rows; rr += BR) {
+    __syncthreads();
+    sq.store(smem);
+    sg.store(smem + TB);
+    if (threadIdx.x < 2 * BR) st[threadIdx.x / BR][threadIdx.x & (BR - 1)] = stat;
+    __syncthreads();
+    if (rr + BR < rows) fetch(rr + BR);
+#pragma unroll 1
+    for (int j = 0; j < BR; j += 32) {
+      const long rj = rr + j;
+      if (rj >= rows) break;
+      const char* tq = smem + j * L::ROWB;
+      const char* tg = tq + TB;
+      f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+      for (int i = 0; i < L::NS; ++i) {
+        s = mma16(view.rows(tq, i), kf[i], s);
+        dp = mma16(view.rows(tg, i), vf[i], dp);
+      }
+      const bool edge = rj + 32 > rows || (int)(rj / G) < wave_last;
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const f32x4 le = *(const f32x4*)&st[0][j + 8 * y + 4 * h];
+        const f32x4 dl = *(const f32x4*)&st[1][j + 8 * y + 4 * h];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          float p = __builtin_amdgcn_exp2f(fmaf(s[4 * y + x], c2, le[x]));
+          if (edge) {
+            const long at = rj + 8 * y + 4 * h + x;
+            if (at >= rows || (int)(at / G) < first_mine) p = 0.f;
+          }
+          s[4 * y + x] = p;
+          dp[4 * y + x] = p * (dp[4 * y + x] - dl[x]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const Frag<T> p = from_acc<T>(s, i), ds = from_acc<T>(dp, i);
+#pragma unroll
+        for (int dt = 0; dt < L::NDT; ++dt) {
+          dv[dt] = mma16(view.cols(tg + 16 * i * L::ROWB, dt), p, dv[dt]);
+          dk[dt] = mma16(view.cols(tq + 16 * i * L::ROWB, dt), ds, dk[dt]);
+        }
+      }
+    }
+  }
+  if (real) {
+    const long at = (krow * a.hkv + kvh) * a.d;
+    store_row<T, DP>((T*)a.dv + at, a.d, h, dv, 1.f);
+    store_row<T, DP>((T*)a.dk + at, a.d, h, dk, a.scale);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+bool aligned(const void* p, long row, long head, int es) {
+  return p != nullptr && ((uintptr_t)p & 15) == 0 && (row * es) % 16 == 0 && (head * es) % 16 == 0 && row >= 0 && head >= 0;
+}
+
+int check_args(const hv_attn_packed_args* a) {
+  if (a == nullptr || (a->dtype != HV_F32 && a->dtype != HV_BF16)) return HV_EINVAL;
+  if (a->hq <= 0 || a->hkv <= 0 || a->hq % a->hkv || a->nseq < 0 || a->total_q < 0 || a->total_k < 0) return HV_EINVAL;
+  if (!(a->scale > 0.f) || a->scale > 3.0e38f || a->cu_q == nullptr || a->cu_k == nullptr) return HV_EINVAL;
+  if (a->d <= 0 || a->d % 8 || a->d > 128 || a->hq > 1024) return HV_EUNSUPPORTED;
+  if (a->total_q >= (1L << 30) || a->total_k >= (1L << 30)) return HV_EUNSUPPORTED;
+  const int es = a->dtype == HV_BF16 ? 2 : 4;
+  if (a->total_q && (!aligned(a->q, a->q_row, a->q_head, es))) return HV_EINVAL;
+  if (a->total_k && (!aligned(a->k, a->k_row, a->k_head, es) || !aligned(a->v, a->v_row, a->v_head, es))) return HV_EINVAL;
+  return HV_OK;
+}
+
+constexpr long MAX_BLOCKS = 1L << 24;                    // a grid stays below 2^32 threads
+
+// blocks that cover `total` rows in nseq sequences and the two ranges outside of them, BM packed rows each
+long tile_bound(long total, int nseq, int G, int BM) { return total * G / BM + nseq + 2; }
+
+template <typename T, int DP> void launch_forward(const hv_attn_packed_args& a, unsigned blocks, hipStream_t s) {
+  if (a.lse != nullptr || a.out_low != nullptr) k_attn_packed<T, DP, true><<<blocks, NT, 0, s>>>(a);
+  else k_attn_packed<T, DP, false><<<blocks, NT, 0, s>>>(a);
+}
+
+template <typename T, int DP>
+void launch_backward(const hv_attn_packed_args& a, unsigned bq, unsigned bk, float* delta, hipStream_t s) {
+  if (a.total_q) {
+    k_attn_packed_delta<T><<<(unsigned)min((a.total_q * a.hq + 3) / 4, 1L << 20), NT, 0, s>>>(a, delta);
+    if (a.dq) k_attn_packed_dq<T, DP><<<bq, NT, 0, s>>>(a, delta);
+  }
+  if (a.total_k && a.dk) k_attn_packed_dkv<T, DP><<<bk, NT, 0, s>>>(a, delta);
+}
+
+// the tile width for a head dimension: the next of 32 / 64 / 128
+#define HV_HEAD_DIM(d, CALL, ...)                  \
+  do {                                             \
+    if ((d) <= 32) CALL<T, 32>(__VA_ARGS__);       \
+    else if ((d) <= 64) CALL<T, 64>(__VA_ARGS__);  \
+    else CALL<T, 128>(__VA_ARGS__);                \
+  } while (0)
+
+}  // namespace
+
+extern "C" size_t hv_attn_packed_args_bytes(void) { return sizeof(hv_attn_packed_args); }
+
+extern "C" size_t hv_attn_packed_work_bytes(const hv_attn_packed_args*) { return 0; }
+
+extern "C" int hv_attn_packed(const hv_attn_packed_args* a, hv_stream_t stream) {
+  const int rc = check_args(a);
+  if (rc != HV_OK) return rc;
+  if (a->total_q == 0) return HV_OK;
+  if (a->out == nullptr || ((uintptr_t)a->out & 15) || ((uintptr_t)a->out_low & 15)) return HV_EINVAL;
+  const long blocks = tile_bound(a->total_q, a->nseq, a->hq / a->hkv, 128) * a->hkv;
+  if (blocks >= MAX_BLOCKS) return HV_EUNSUPPORTED;
+  hipStream_t s = (hipStream_t)stream;
+  HV_DISPATCH(a->dtype, HV_HEAD_DIM(a->d, launch_forward, *a, (unsigned)blocks, s));
+  HV_CHECK_LAUNCH();
+  hv_diag_count(HV_KF_ATTN_PACKED);
+  return HV_OK;
+}
+
+extern "C" size_t hv_attn_packed_backward_work_bytes(const hv_attn_packed_args* a) {
+  return a == nullptr || a->total_q <= 0 || a->hq <= 0 ? 0 : (size_t)a->total_q * a->hq * sizeof(float);
+}
+
+extern "C" int hv_attn_packed_backward(const hv_attn_packed_args* a, hv_stream_t stream) {
+  const int rc = check_args(a);
+  if (rc != HV_OK) return rc;
+  const int es = a->dtype == HV_BF16 ? 2 : 4;
+  if (a->total_q && (!aligned(a->dout, a->do_row, a->do_head, es) || a->out == nullptr || a->lse == nullptr ||
+                     ((uintptr_t)a->dq & 15) || a->work == nullptr))
+    return HV_EINVAL;
+  if ((a->dk == nullptr) != (a->dv == nullptr) || ((uintptr_t)a->dk & 15) || ((uintptr_t)a->dv & 15)) return HV_EINVAL;
+  const long bq = tile_bound(a->total_q, a->nseq, a->hq / a->hkv, 128) * a->hkv;
+  const long bk = tile_bound(a->total_k, a->nseq, 1, 128) * a->hkv;
+  if (bq >= MAX_BLOCKS || bk >= MAX_BLOCKS) return HV_EUNSUPPORTED;
+  hipStream_t s = (hipStream_t)stream;
+  HV_DISPATCH(a->dtype, HV_HEAD_DIM(a->d, launch_backward, *a, (unsigned)bq, (unsigned)bk, (float*)a->work, s));
+  HV_CHECK_LAUNCH();
+  hv_diag_count(HV_KF_ATTN_PACKED);
+  return HV_OK;
+}

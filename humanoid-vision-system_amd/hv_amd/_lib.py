@@ -14,7 +14,7 @@ import threading
 
 import torch  # noqa: F401  (must be loaded first: HIP runtime shared by soname)
 
-HV_F32, HV_BF16 = 0, 1
+HV_F32, HV_BF16, HV_E4M3 = 0, 1, 3
 # per-call kernel variants (include/hv_kernels.h HV_GV_* / HV_MV_*): 0 = automatic
 GV_TILE_128x128, GV_TILE_64x128, GV_TILE_128x64, GV_TILE_64x64, GV_TILE_256, GV_TILE_SMALLK = 1, 2, 3, 4, 5, 6
 GV_REGSTAGE, GV_NO_BIG, GV_BIG_ALWAYS, GV_NO_SMALL = 0x8, 0x10, 0x20, 0x40
@@ -142,6 +142,14 @@ class WprepEntry(C.Structure):
                 ("eps", f32), ("pad_", i32)]
 
 
+class AttnPackedArgs(C.Structure):
+    _fields_ = [("dtype", i32), ("hq", i32), ("hkv", i32), ("d", i32), ("nseq", i32), ("causal", i32),
+                ("scale", f32), ("pad_", i32), ("total_q", i64), ("total_k", i64), ("cu_q", vp), ("cu_k", vp),
+                ("q", vp), ("k", vp), ("v", vp), ("q_row", i64), ("q_head", i64), ("k_row", i64), ("k_head", i64),
+                ("v_row", i64), ("v_head", i64), ("out", vp), ("out_low", vp), ("lse", vp), ("work", vp),
+                ("dout", vp), ("do_row", i64), ("do_head", i64), ("dq", vp), ("dk", vp), ("dv", vp)]
+
+
 _SIGS = {
     "hv_mhc_prep_scratch_floats": ([i32, i32], C.c_size_t),
     "hv_mhc_prep_blocks": ([i32, i32, i32, vp], None),
@@ -252,6 +260,18 @@ _SIGS = {
     "hv_grad_norms": ([vp, i32, i32, i32, vp, vp, vp, vp, vp, vp], i32),
     "hv_adamw": ([vp, i32, i32, vp, f32, f32, f32, f32, f32, i32, vp, vp, vp], i32),
     "hv_adamw_dev": ([vp, i32, i32, vp, vp, vp, vp, vp], i32),
+    # ---- sequence operators
+    "hv_attn_packed_args_bytes": ([], C.c_size_t),
+    "hv_attn_packed_work_bytes": ([vp], C.c_size_t),
+    "hv_attn_packed": ([vp, vp], i32),
+    "hv_attn_packed_backward_work_bytes": ([vp], C.c_size_t),
+    "hv_attn_packed_backward": ([vp, vp], i32),
+    "hv_add_rmsnorm": ([i32, vp, i32, vp, i64, i32, f32, vp, vp, i32, vp, vp, vp, vp], i32),
+    "hv_add_rmsnorm_backward_work_floats": ([i64, i32], C.c_size_t),
+    "hv_add_rmsnorm_backward": ([i32, vp, vp, vp, i32, vp, vp, i64, i32, i32, vp, vp, vp, vp, vp], i32),
+    "hv_quantize_rows_fp8": ([i32, vp, i64, i64, i32, vp, vp, vp], i32),
+    "hv_linear_fp8_work_bytes": ([i64, i32, i32], C.c_size_t),
+    "hv_linear_fp8": ([vp, i64, vp, vp, i64, vp, vp, i32, i64, i32, i32, i32, vp, i64, vp, vp], i32),
 }
 
 EXPORTED = tuple(_SIGS)
@@ -267,6 +287,9 @@ def _declare(lib):
     want = [C.sizeof(s) for s in (SinkhornEntry, GemmDesc, MhcFusedArgs, MhcPrepEntry, WprepEntry)]
     if list(sizes) != want:
         raise RuntimeError(f"libhvs struct layout mismatch: C {list(sizes)} vs ctypes {want}")
+    if lib.hv_attn_packed_args_bytes() != C.sizeof(AttnPackedArgs):
+        raise RuntimeError(f"libhvs struct layout mismatch: hv_attn_packed_args is {lib.hv_attn_packed_args_bytes()} "
+                           f"bytes, the binding's {C.sizeof(AttnPackedArgs)}")
 
 
 def lib():

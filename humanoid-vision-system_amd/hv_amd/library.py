@@ -20,6 +20,11 @@ Ops (reference function each replaces):
   hv::attention      softmax(QK^T/sqrt(hd)) V                manifold_layers.py:404-427
   hv::layernorm      nn.LayerNorm                            manifold_layers.py:250,267
   hv::rmsnorm        RMSNorm.forward                         manifold_layers.py:449-456
+  hv::attention_packed  the same core over packed sequences of different lengths, grouped heads, causal
+  hv::add_rmsnorm    residual addition + RMSNorm.forward     vit_encoder_decoder.py:190-208, manifold_layers.py:449-456
+  hv::add_rmsnorm_fp8   the same with 8-bit rows (inference)
+  hv::quantize_rows_fp8 rows (a weight) in 8 bits            -
+  hv::linear_fp8     nn.Linear + activation on 8-bit rows    vit_encoder_decoder.py:146-152
   hv::yolo_decode    YOLODecoder.forward (+S5)               yolo_head.py:220-294
   hv::nms            post_process + non_max_suppression      yolo_head.py:571-731
 """
@@ -243,6 +248,102 @@ def _attn_bwd(ctx, do):
 attention.register_autograd(_attn_bwd, setup_context=_attn_setup)
 
 
+# ----------------------------------------------------------------------------------- packed attention
+@torch.library.custom_op("hv::attention_packed", mutates_args=(), device_types="cuda")
+def attention_packed(q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Tensor, causal: bool = False,
+                     scale: Optional[float] = None) -> Tuple[Tensor, Tensor]:
+    """q [rows, heads, d], k / v [rows, kv heads, d], offsets int32 [sequences + 1] -> (out like q, log-sum-exp
+    [rows, heads] fp32, not differentiable); see ops.attention_packed."""
+    fit = [t if t.dim() != 3 or ops.rows_dense(t) else t.contiguous() for t in (q, k, v)]
+    return ops.attention_packed(*fit, cu_q, cu_k, causal=causal, scale=scale, return_lse=True)
+
+
+@attention_packed.register_fake
+def _(q, k, v, cu_q, cu_k, causal=False, scale=None):
+    return q.new_empty(q.shape), q.new_empty(q.shape[:2], dtype=torch.float32)
+
+
+def _attn_packed_setup(ctx, inputs, output):
+    q, k, v, cu_q, cu_k, causal, scale = inputs
+    ctx.save_for_backward(q, k, v, cu_q, cu_k)
+    ctx.meta = (causal, scale)
+
+
+def _attn_packed_bwd(ctx, do, dlse):
+    from .train_fn import attention_packed as packed
+    q, k, v, cu_q, cu_k = ctx.saved_tensors
+    causal, scale = ctx.meta
+    g = _grad_of(lambda a, b, c: packed(a, b, c, cu_q, cu_k, causal=causal, scale=scale), [q, k, v], [do])
+    return g[0], g[1], g[2], None, None, None, None
+
+
+attention_packed.register_autograd(_attn_packed_bwd, setup_context=_attn_packed_setup)
+
+
+# ----------------------------------------------------------------------------------- residual + norm, 8-bit rows
+@torch.library.custom_op("hv::add_rmsnorm", mutates_args=(), device_types="cuda")
+def add_rmsnorm(x: Tensor, residual: Tensor, scale: Tensor, eps: float = 1e-8) -> Tuple[Tensor, Tensor]:
+    """(RMSNorm(x + residual) * scale in x's dtype, x + residual in residual's)."""
+    return ops.add_rmsnorm(x.contiguous(), residual.contiguous(), ops.f32(scale), eps)
+
+
+@add_rmsnorm.register_fake
+def _(x, residual, scale, eps=1e-8):
+    return x.new_empty(x.shape), residual.new_empty(residual.shape)
+
+
+def _add_rms_setup(ctx, inputs, output):
+    x, residual, scale, eps = inputs
+    ctx.save_for_backward(x, residual, scale)
+    ctx.eps = eps
+
+
+def _add_rms_bwd(ctx, dy, ds):
+    from .train_fn import AddRMSNormFn
+    eps = ctx.eps
+    fn = lambda x, r, w: AddRMSNormFn.apply(x.contiguous(), r.contiguous(), w, eps, None)     # noqa: E731
+    g = _grad_of(fn, list(ctx.saved_tensors), [dy, ds])
+    return g[0], g[1], g[2], None
+
+
+add_rmsnorm.register_autograd(_add_rms_bwd, setup_context=_add_rms_setup)
+
+
+@torch.library.custom_op("hv::add_rmsnorm_fp8", mutates_args=(), device_types="cuda")
+def add_rmsnorm_fp8(x: Tensor, residual: Tensor, scale: Tensor, eps: float = 1e-8) -> Tuple[Tensor, Tensor, Tensor]:
+    """(e4m3 codes, row scale, x + residual): RMSNorm(x + residual) * scale ~ codes * row scale.  Inference."""
+    return ops.add_rmsnorm_fp8(x.contiguous(), residual.contiguous(), ops.f32(scale), eps)
+
+
+@add_rmsnorm_fp8.register_fake
+def _(x, residual, scale, eps=1e-8):
+    return (x.new_empty(x.shape, dtype=torch.float8_e4m3fn), x.new_empty(x.shape[:-1], dtype=torch.float32),
+            residual.new_empty(residual.shape))
+
+
+@torch.library.custom_op("hv::quantize_rows_fp8", mutates_args=(), device_types="cuda")
+def quantize_rows_fp8(x: Tensor) -> Tuple[Tensor, Tensor]:
+    """x [rows, cols] -> (e4m3 codes, row scale): x ~ codes * row scale."""
+    return ops.quantize_rows_fp8(x.contiguous())
+
+
+@quantize_rows_fp8.register_fake
+def _(x):
+    return x.new_empty(x.shape, dtype=torch.float8_e4m3fn), x.new_empty(x.shape[:1], dtype=torch.float32)
+
+
+@torch.library.custom_op("hv::linear_fp8", mutates_args=(), device_types="cuda")
+def linear_fp8(a: Tensor, a_scale: Tensor, w: Tensor, w_scale: Tensor, bias: Optional[Tensor] = None,
+               act: str = "none", out_dtype: torch.dtype = torch.bfloat16) -> Tensor:
+    """act((a_scale * a) (w_scale * w)^T + bias) on e4m3 rows a [m, k], w [n, k].  Inference."""
+    return ops.linear_fp8(a, a_scale, w, w_scale, bias=ops.f32(bias), act=act, out_dtype=out_dtype)
+
+
+@linear_fp8.register_fake
+def _(a, a_scale, w, w_scale, bias=None, act="none", out_dtype=torch.bfloat16):
+    return a.new_empty((a.shape[0], w.shape[0]), dtype=out_dtype)
+
+
 # ----------------------------------------------------------------------------------- norms
 @torch.library.custom_op("hv::layernorm", mutates_args=(), device_types="cuda")
 def layernorm(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], eps: float = 1e-5) -> Tensor:
@@ -338,5 +439,5 @@ def _(boxes, class_scores, class_indices, conf_threshold, iou_threshold, max_det
             boxes[0].new_empty((B,), dtype=torch.int32))
 
 
-OPS = ("sinkhorn", "mhc", "linear", "conv_bn_act", "se_gate", "attention", "layernorm", "rmsnorm", "yolo_decode",
-       "nms")
+OPS = ("sinkhorn", "mhc", "linear", "conv_bn_act", "se_gate", "attention", "attention_packed", "layernorm",
+       "rmsnorm", "add_rmsnorm", "add_rmsnorm_fp8", "quantize_rows_fp8", "linear_fp8", "yolo_decode", "nms")

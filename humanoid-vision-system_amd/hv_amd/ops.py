@@ -795,6 +795,206 @@ def attention_general(q: Tensor, k: Tensor, v: Tensor, heads: int, key_padding_m
     return o, w
 
 
+# ---------------------------------------------------------------------------- sequence operators
+class on_device:
+    """Launch on `t`'s device and its current stream, also where another device is the current one."""
+
+    def __init__(self, t: Tensor):
+        self.index = t.device.index
+        self.guard = None
+
+    def __enter__(self):
+        if self.index != torch.cuda.current_device():
+            self.guard = torch.cuda.device(self.index)
+            self.guard.__enter__()
+        return stream_ptr()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+        return False
+
+
+def _same_device(what: str, first: Tensor, *others) -> None:
+    _cuda(first, *others)
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{what}: tensors on {first.device} and {t.device}")
+
+
+def rows_dense(t: Tensor) -> bool:
+    """Whether attention_packed can read `t` [rows, heads, d] in place: last dimension dense, every row
+    start on a 16-byte boundary."""
+    es = t.element_size()
+    return (t.stride(2) == 1 or t.shape[2] == 1) and t.data_ptr() % 16 == 0 and \
+        (t.stride(0) * es) % 16 == 0 and (t.stride(1) * es) % 16 == 0
+
+
+def attn_packed_args(q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Tensor, causal: bool,
+                     scale: Optional[float]) -> L.AttnPackedArgs:
+    """Check the operands of a packed attention and describe them (hv_attn_packed_args)."""
+    _same_device("attention_packed", q, k, v, cu_q, cu_k)
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        raise ValueError("attention_packed: q is [rows, heads, d], k and v are [rows, kv heads, d]")
+    hq, d = q.shape[1], q.shape[2]
+    hkv = k.shape[1]
+    if k.shape != v.shape or k.shape[2] != d or q.dtype != k.dtype or q.dtype != v.dtype:
+        raise ValueError(f"attention_packed: q {tuple(q.shape)} {q.dtype}, k {tuple(k.shape)} {k.dtype}, "
+                         f"v {tuple(v.shape)} {v.dtype} disagree")
+    if hkv == 0 or hq == 0 or hq % hkv:
+        raise ValueError(f"attention_packed: {hq} query heads do not share {hkv} key / value heads")
+    if d == 0 or d % 8 or d > 128 or hq > 1024:
+        raise ValueError(f"attention_packed: head dim {d} (a multiple of 8 up to 128), {hq} heads (up to 1024)")
+    if cu_q.dtype != torch.int32 or cu_k.dtype != torch.int32 or cu_q.dim() != 1 or cu_q.shape != cu_k.shape or \
+            cu_q.numel() == 0 or not cu_q.is_contiguous() or not cu_k.is_contiguous():
+        raise ValueError("attention_packed: cu_q and cu_k are int32 offsets [sequences + 1]")
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t.numel() and not rows_dense(t):
+            raise ValueError(f"attention_packed: {name} needs a dense last dimension and 16-byte aligned rows "
+                             f"(strides {t.stride()})")
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < 3e38:
+        raise ValueError(f"attention_packed: scale {scale} is not a positive finite number")
+    a = L.AttnPackedArgs()
+    a.dtype, a.hq, a.hkv, a.d, a.nseq, a.causal = dtype_code(q.dtype), hq, hkv, d, cu_q.numel() - 1, int(bool(causal))
+    a.scale, a.total_q, a.total_k = scale, q.shape[0], k.shape[0]
+    a.cu_q, a.cu_k = cu_q.data_ptr(), cu_k.data_ptr()
+    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    a.q_row, a.q_head = q.stride(0), q.stride(1)
+    a.k_row, a.k_head = k.stride(0), k.stride(1)
+    a.v_row, a.v_head = v.stride(0), v.stride(1)
+    return a
+
+
+def attention_packed(q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Optional[Tensor] = None, *,
+                     causal: bool = False, scale: Optional[float] = None, return_lse: bool = False):
+    """softmax(scale q k^T) v over packed sequences of different lengths.
+
+    q [rows, heads, d], k / v [rows, kv heads, d] (bf16 or fp32; rows and heads may lie apart), heads a
+    multiple of kv heads (query head h reads kv head h * kv heads // heads).  Sequence s owns the query rows
+    cu_q[s] .. cu_q[s+1]-1 and the key rows cu_k[s] .. cu_k[s+1]-1 (int32 on the device, ascending; cu_k
+    defaults to cu_q).  causal: query i of a sequence sees its keys up to i + (keys - queries), so one new
+    token against a history is a sequence of one query.  scale defaults to d ** -0.5.
+
+    Returns out [rows, heads, d] (with return_lse also the log-sum-exp [rows, heads], fp32).  Rows that see no
+    key and rows of no sequence are 0 (lse -inf).  Rows of other sequences never enter a result, whatever they
+    hold; inside a sequence the values are finite (a key that the causal mask hides is multiplied by 0)."""
+    cu_k = cu_q if cu_k is None else cu_k
+    a = attn_packed_args(q, k, v, cu_q, cu_k, causal, scale)
+    out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    lse = torch.empty(q.shape[:2], device=q.device, dtype=torch.float32) if return_lse else None
+    lib = L.lib()
+    with on_device(q) as stream:
+        a.out, a.lse = out.data_ptr(), ptr(lse)
+        n = lib.hv_attn_packed_work_bytes(C.byref(a))
+        work = torch.empty(n, device=q.device, dtype=torch.uint8) if n else None
+        a.work = ptr(work)
+        check(lib.hv_attn_packed(C.byref(a), stream), "hv_attn_packed")
+    return (out, lse) if return_lse else out
+
+
+def norm_operands(what: str, x: Tensor, residual: Optional[Tensor], scale: Tensor):
+    """(rows, cols) of a residual addition + norm, after the checks of its operands."""
+    _same_device(what, x, residual, scale)
+    if x.dim() == 0 or x.shape[-1] == 0 or scale.shape != x.shape[-1:]:
+        raise ValueError(f"{what}: x {tuple(x.shape)}, scale {tuple(scale.shape)}: scale is [x.shape[-1]]")
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"{what}: x {tuple(x.shape)} and residual {tuple(residual.shape)} disagree")
+    for name, t in (("x", x), ("residual", residual), ("scale", scale)):
+        if t is not None:
+            _contig(t, f"{what} {name}")
+    if scale.dtype != torch.float32:
+        raise TypeError(f"{what}: scale is fp32, got {scale.dtype}")
+    cols = x.shape[-1]
+    if cols > 32768:
+        raise ValueError(f"{what}: {cols} columns (32768 at most)")
+    return x.numel() // cols, cols
+
+
+def _add_rmsnorm(what, x, residual, scale, eps, y, y_code, y_scale, rstd=None):
+    rows, cols = norm_operands(what, x, residual, scale)
+    s = torch.empty_like(residual) if residual is not None else None
+    with on_device(x) as stream:
+        check(L.lib().hv_add_rmsnorm(dtype_code(x.dtype), x.data_ptr(),
+                                     dtype_code(residual.dtype) if residual is not None else 0, ptr(residual), rows,
+                                     cols, eps, scale.data_ptr(), ptr(s), y_code, y.data_ptr(), ptr(y_scale),
+                                     ptr(rstd), stream), "hv_add_rmsnorm")
+    return s
+
+
+def add_rmsnorm(x: Tensor, residual: Tensor, scale: Tensor, eps: float = 1e-8,
+                out_dtype: Optional[torch.dtype] = None):
+    """s = x + residual, y = s / sqrt(mean(s^2) + eps) * scale over the last dimension in one pass: (y, s).
+
+    s has residual's dtype (an fp32 residual stream stays fp32), y out_dtype (default x's); the sum is
+    normalised before it is rounded."""
+    y = torch.empty(x.shape, device=x.device, dtype=out_dtype or x.dtype)
+    s = _add_rmsnorm("add_rmsnorm", x, residual, scale, eps, y, dtype_code(y.dtype), None)
+    return y, s
+
+
+def add_rmsnorm_fp8(x: Tensor, residual: Optional[Tensor], scale: Tensor, eps: float = 1e-8):
+    """add_rmsnorm with y in 8 bits: (codes e4m3 [..., cols], row scale fp32 [...], s), y ~ codes * row scale,
+    row scale = max(row maximum of |y| / 448, 2^-120): the operand of linear_fp8.  residual None: s is None
+    and x itself is normalised."""
+    codes = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn)
+    row_scale = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
+    s = _add_rmsnorm("add_rmsnorm_fp8", x, residual, scale, eps, codes, L.HV_E4M3, row_scale)
+    return codes, row_scale, s
+
+
+def quantize_rows_fp8(x: Tensor):
+    """x [rows, cols] (rows may lie apart) -> (codes e4m3 [rows, cols], row scale fp32 [rows]) with
+    x ~ codes * row scale: lays a weight [out, in] out for linear_fp8 once."""
+    _cuda(x)
+    if x.dim() != 2 or x.shape[1] == 0 or x.shape[1] > 32768:
+        raise ValueError(f"quantize_rows_fp8: x {tuple(x.shape)} is not [rows, 1 .. 32768 columns]")
+    if x.stride(1) != 1 and x.shape[1] > 1 or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
+        raise ValueError("quantize_rows_fp8: rows must be dense")
+    codes = torch.empty(x.shape, device=x.device, dtype=torch.float8_e4m3fn)
+    scale = torch.empty(x.shape[0], device=x.device, dtype=torch.float32)
+    with on_device(x) as stream:
+        check(L.lib().hv_quantize_rows_fp8(dtype_code(x.dtype), x.data_ptr(), max(x.stride(0), x.shape[1]), x.shape[0],
+                                           x.shape[1], codes.data_ptr(), scale.data_ptr(), stream),
+              "hv_quantize_rows_fp8")
+    return codes, scale
+
+
+def linear_fp8(a: Tensor, a_scale: Tensor, w: Tensor, w_scale: Tensor, *, bias: Optional[Tensor] = None,
+               act: str = "none", out_dtype: torch.dtype = torch.bfloat16) -> Tensor:
+    """act((a_scale * a) (w_scale * w)^T + bias) for 8-bit rows a [m, k], w [n, k] (e4m3 codes with an fp32 scale
+    per row: add_rmsnorm_fp8, quantize_rows_fp8) -> [m, n] bf16 or fp32.  Sums, scales and activation are fp32."""
+    _same_device("linear_fp8", a, a_scale, w, w_scale, bias)
+    f8 = torch.float8_e4m3fn
+    if a.dtype != f8 or w.dtype != f8 or a.dim() != 2 or w.dim() != 2 or a.shape[1] != w.shape[1]:
+        raise ValueError(f"linear_fp8: a {tuple(a.shape)} {a.dtype} and w {tuple(w.shape)} {w.dtype} are not e4m3 "
+                         "[m, k] and [n, k]")
+    m, k = a.shape
+    n = w.shape[0]
+    for name, t, want in (("a_scale", a_scale, m), ("w_scale", w_scale, n), ("bias", bias, n)):
+        if t is not None and (tuple(t.shape) != (want,) or t.dtype != torch.float32 or not t.is_contiguous()):
+            raise ValueError(f"linear_fp8: {name} {tuple(t.shape)} {t.dtype} is not dense fp32 [{want}]")
+    for name, t in (("a", a), ("w", w)):
+        if t.numel() and (k % 16 or t.stride(1) != 1 or t.data_ptr() % 16 or
+                          (t.shape[0] > 1 and (t.stride(0) % 16 or t.stride(0) < k))):
+            raise ValueError(f"linear_fp8: {name} needs k a multiple of 16 and dense, 16-byte aligned rows "
+                             f"(shape {tuple(t.shape)}, strides {t.stride()})")
+    if k == 0:
+        raise ValueError("linear_fp8: k is 0")
+    if act not in L.ACT:
+        raise ValueError(f"linear_fp8: unknown activation {act!r}")
+    out_code = dtype_code(out_dtype)
+    out = torch.empty((m, n), device=a.device, dtype=out_dtype)
+    lib = L.lib()
+    nb = lib.hv_linear_fp8_work_bytes(m, n, k)
+    work = torch.empty(nb, device=a.device, dtype=torch.uint8) if nb else None
+    with on_device(a) as stream:
+        check(lib.hv_linear_fp8(a.data_ptr(), a.stride(0) if m > 1 else k, a_scale.data_ptr(), w.data_ptr(),
+                                w.stride(0) if n > 1 else k, w_scale.data_ptr(), ptr(bias), L.ACT[act], m, n, k,
+                                out_code, out.data_ptr(), n, ptr(work), stream), "hv_linear_fp8")
+    return out
+
+
 def gather_rows(x: Tensor, stride_rows: int) -> Tensor:
     """Row 0 of every group of `stride_rows` rows: x [n*stride_rows, c] -> [n, c]."""
     c = x.shape[-1]
@@ -1083,7 +1283,7 @@ def stability_stats(x_in: Tensor, x_out: Tensor, h: Tensor, history: Optional[Te
 # ---------------------------------------------------------------------------- diagnostics
 KERNEL_FAMILIES = ("gemm_pp256", "glds_128x128", "glds_64x128", "glds_128x64", "glds_64x64", "gemm_regstage",
                    "mhc_fused", "attn_mfma", "attn_scalar", "sinkhorn_group", "attn_general", "gemm_smallk",
-                   "gemm_splitk")
+                   "gemm_splitk", "attn_packed", "add_rmsnorm", "linear_fp8")
 
 
 def launch_counts(reset: bool = False) -> dict:
@@ -1107,7 +1307,8 @@ def _install_sync_check():
     for name in ("gemm", "conv2d", "conv_weight_prep", "bn_fold", "cast", "row_stats", "layernorm", "rmsnorm",
                  "sinkhorn", "mhc_prep", "nchw_to_nhwc", "maxpool2x2", "channel_mean", "se_mlp", "se_gate",
                  "scale_residual", "upsample_add", "add_scaled", "add_rowvec", "interp_linear", "vit_tokens",
-                 "attention", "gather_rows", "yolo_decode"):
+                 "attention", "attention_packed", "add_rmsnorm", "add_rmsnorm_fp8", "quantize_rows_fp8", "linear_fp8",
+                 "gather_rows", "yolo_decode"):
         fn = getattr(mod, name)
 
         def wrap(fn=fn, name=name):

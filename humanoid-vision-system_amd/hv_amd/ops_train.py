@@ -14,7 +14,7 @@ from torch.autograd.graph import increment_version
 
 from . import _lib as L
 from ._lib import check, dtype_code, ptr, stream_ptr
-from .ops import _contig, _cuda, f32
+from .ops import _contig, _cuda, attn_packed_args, f32, norm_operands, on_device, rows_dense
 from .runtime import options, seed_offset_ptr
 
 Tensor = torch.Tensor
@@ -483,6 +483,86 @@ def attention_backward(q, k, v, o, do, lse, heads: int, drop_p: float, seed: int
                                         dk.data_ptr(),
                                         dv.data_ptr(), work.data_ptr(), stream_ptr()), "hv_attention_backward")
     return dq, dk, dv
+
+
+def attention_packed_train(q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Tensor, causal: bool,
+                           scale: Optional[float]):
+    """ops.attention_packed with what its backward needs: (out, out_low, lse).  out_low (bf16 only) is the part
+    of out that its rounding cut off: the backward's row mean dO . O would otherwise carry that rounding into
+    every score gradient of the row."""
+    a = attn_packed_args(q, k, v, cu_q, cu_k, causal, scale)
+    out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    low = torch.empty_like(out) if q.dtype == torch.bfloat16 else None
+    lse = torch.empty(q.shape[:2], device=q.device, dtype=torch.float32)
+    lib = L.lib()
+    with on_device(q) as stream:
+        a.out, a.out_low, a.lse = out.data_ptr(), ptr(low), lse.data_ptr()
+        n = lib.hv_attn_packed_work_bytes(C.byref(a))
+        work = torch.empty(n, device=q.device, dtype=torch.uint8) if n else None
+        a.work = ptr(work)
+        check(lib.hv_attn_packed(C.byref(a), stream), "hv_attn_packed")
+    return out, low, lse
+
+
+def attention_packed_backward(q, k, v, cu_q, cu_k, causal: bool, scale: Optional[float], out, low, lse, dout,
+                              need_q: bool = True, need_kv: bool = True):
+    """(dq, dk, dv) of attention_packed_train, dense; the ones that are not needed are None."""
+    if dout.shape != q.shape or dout.dtype != q.dtype:
+        raise ValueError(f"attention_packed_backward: dout {tuple(dout.shape)} {dout.dtype} is not like q")
+    a = attn_packed_args(q, k, v, cu_q, cu_k, causal, scale)
+    if dout.numel() and not rows_dense(dout):
+        dout = dout.contiguous()
+    dq = torch.empty(q.shape, device=q.device, dtype=q.dtype) if need_q else None
+    dk = torch.empty(k.shape, device=q.device, dtype=q.dtype) if need_kv else None
+    dv = torch.empty(v.shape, device=q.device, dtype=q.dtype) if need_kv else None
+    lib = L.lib()
+    with on_device(q) as stream:
+        a.out, a.out_low, a.lse = out.data_ptr(), ptr(low), lse.data_ptr()
+        a.dout, a.do_row, a.do_head = dout.data_ptr(), dout.stride(0), dout.stride(1)
+        a.dq, a.dk, a.dv = ptr(dq), ptr(dk), ptr(dv)
+        work = torch.empty(lib.hv_attn_packed_backward_work_bytes(C.byref(a)), device=q.device, dtype=torch.uint8)
+        a.work = work.data_ptr()
+        check(lib.hv_attn_packed_backward(C.byref(a), stream), "hv_attn_packed_backward")
+    return dq, dk, dv
+
+
+def add_rmsnorm_train(x: Tensor, residual: Tensor, scale: Tensor, eps: float, out_dtype: Optional[torch.dtype] = None):
+    """ops.add_rmsnorm with the row factors that its backward needs: (y, s, rstd)."""
+    rows, cols = norm_operands("add_rmsnorm", x, residual, scale)
+    y = torch.empty(x.shape, device=x.device, dtype=out_dtype or x.dtype)
+    s = torch.empty_like(residual)
+    rstd = torch.empty(rows, device=x.device, dtype=torch.float32)
+    with on_device(x) as stream:
+        check(L.lib().hv_add_rmsnorm(dtype_code(x.dtype), x.data_ptr(), dtype_code(residual.dtype), residual.data_ptr(),
+                                     rows, cols, eps, scale.data_ptr(), s.data_ptr(), dtype_code(y.dtype), y.data_ptr(),
+                                     None, rstd.data_ptr(), stream), "hv_add_rmsnorm")
+    return y, s, rstd
+
+
+def add_rmsnorm_backward(s: Tensor, rstd: Tensor, scale: Tensor, dy: Tensor, ds: Optional[Tensor],
+                         dx_dtype: Optional[torch.dtype], need_residual: bool = True):
+    """(dx, dresidual, dscale) of add_rmsnorm_train: dx and dresidual are one value in two dtypes -- the same
+    tensor where the dtypes agree; dx_dtype None / need_residual False: not wanted."""
+    _contig(s, "s")
+    _contig(dy, "dy")
+    if ds is not None and (ds.shape != s.shape or ds.dtype != s.dtype or not ds.is_contiguous()):
+        raise ValueError("add_rmsnorm_backward: ds is not like s")
+    if dy.shape != s.shape:
+        raise ValueError("add_rmsnorm_backward: dy and s disagree")
+    cols = s.shape[-1]
+    rows = s.numel() // cols
+    shared = dx_dtype == s.dtype
+    dx = torch.empty(s.shape, device=s.device, dtype=dx_dtype) if dx_dtype is not None else None
+    dr = torch.empty_like(s) if need_residual and not shared else None
+    dscale = torch.empty(cols, device=s.device, dtype=torch.float32)
+    lib = L.lib()
+    work = _work(lib.hv_add_rmsnorm_backward_work_floats(rows, cols), s.device)
+    with on_device(s) as stream:
+        check(lib.hv_add_rmsnorm_backward(dtype_code(s.dtype), s.data_ptr(), rstd.data_ptr(), scale.data_ptr(),
+                                          dtype_code(dy.dtype), dy.data_ptr(), ptr(ds), rows, cols,
+                                          dtype_code(dx_dtype) if dx is not None else 0, ptr(dx), ptr(dr),
+                                          dscale.data_ptr(), work.data_ptr(), stream), "hv_add_rmsnorm_backward")
+    return dx, (dx if shared and need_residual else dr), dscale
 
 
 # ---------------------------------------------------------------------------- loss

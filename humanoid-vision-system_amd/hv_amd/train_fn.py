@@ -15,6 +15,8 @@ from typing import List, Optional, Sequence
 
 import torch
 
+from torch.autograd.function import once_differentiable
+
 from . import ops
 from . import ops_train as T
 from .ops import f32
@@ -471,6 +473,66 @@ class AttentionFn(torch.autograd.Function):
         q, k, v, o, lse = ctx.saved_tensors
         dq, dk, dv = T.attention_backward(q, k, v, o, g.contiguous(), lse, heads, p, seed)
         return dq, dk, dv, None, None, None
+
+
+class PackedAttentionFn(torch.autograd.Function):
+    """Attention over packed sequences (ops.attention_packed) with its gradient."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, cu_q, cu_k, causal: bool, scale):
+        out, low, lse = T.attention_packed_train(q, k, v, cu_q, cu_k, causal, scale)
+        ctx.meta = (causal, scale)
+        ctx.save_for_backward(q, k, v, cu_q, cu_k, out, low, lse)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        q, k, v, cu_q, cu_k, out, low, lse = ctx.saved_tensors
+        dq, dk, dv = T.attention_packed_backward(q, k, v, cu_q, cu_k, *ctx.meta, out, low, lse, g, _need(ctx, 0),
+                                                 _need(ctx, 1) or _need(ctx, 2))
+        return dq, dk, dv, None, None, None, None
+
+
+def attention_packed(q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Optional[Tensor] = None, *,
+                     causal: bool = False, scale: Optional[float] = None) -> Tensor:
+    """ops.attention_packed, differentiable in q, k and v.  Inputs that the kernels cannot read in place (last
+    dimension not dense, rows not 16-byte aligned) are copied."""
+    fit = [t if t.dim() != 3 or ops.rows_dense(t) else t.contiguous() for t in (q, k, v)]
+    return PackedAttentionFn.apply(*fit, cu_q, cu_q if cu_k is None else cu_k, bool(causal), scale)
+
+
+class AddRMSNormFn(torch.autograd.Function):
+    """Residual addition + RMS norm (ops.add_rmsnorm) with its gradient: returns (y, s)."""
+
+    @staticmethod
+    def forward(ctx, x, residual, scale, eps: float, out_dtype):
+        w = f32(scale)
+        y, s, rstd = T.add_rmsnorm_train(x, residual, w, eps, out_dtype)
+        ctx.set_materialize_grads(False)
+        ctx.dtypes = (x.dtype, scale.dtype)
+        ctx.save_for_backward(s, rstd, w)
+        return y, s
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, ds):
+        s, rstd, w = ctx.saved_tensors
+        x_dtype, w_dtype = ctx.dtypes
+        if dy is None:                                   # only the sum was used
+            if ds is None:
+                return None, None, None, None, None
+            return ds.to(x_dtype), ds, None, None, None
+        ds = None if ds is None else ds.contiguous()
+        dx, dr, dw = T.add_rmsnorm_backward(s, rstd, w, dy.contiguous(), ds, x_dtype if _need(ctx, 0) else None,
+                                            _need(ctx, 1))
+        return dx, dr, dw.to(w_dtype), None, None
+
+
+def add_rmsnorm(x: Tensor, residual: Tensor, scale: Tensor, eps: float = 1e-8,
+                out_dtype: Optional[torch.dtype] = None):
+    """ops.add_rmsnorm, differentiable: (y, s) with s = x + residual, y = RMSNorm(s) * scale."""
+    return AddRMSNormFn.apply(x.contiguous(), residual.contiguous(), scale, eps, out_dtype)
 
 
 # =============================================================================== loss

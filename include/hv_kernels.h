@@ -741,6 +741,71 @@ int hv_symeig_group(const hv_symeig_entry* dev_table, const int* host_n, int cou
 size_t hv_stability_work_floats(int rows);
 int hv_stability_stats(int dtype, const void* x_in, const void* x_out, int rows, int D, const float* h, int n,
                        float* work, float* history, int slot, float* out3, hv_stream_t stream);
+/* ------------------------------------------------------------------------------------
+ * Sequence operators: attention over packed sequences, residual addition + RMS norm (8-bit
+ * rows, training), linear layer on 8-bit rows.
+ * ------------------------------------------------------------------------------------ */
+/* Attention over packed sequences of different lengths (manifold_layers.py:404-427 computes one
+ * length per batch): sequence s owns query rows cu_q[s] .. cu_q[s+1]-1 and key rows cu_k[s] ..
+ * cu_k[s+1]-1 of the packed tensors.  out_i = sum_j softmax_j(scale q_i . k_j) v_j over the keys j
+ * of the same sequence, with causal != 0 only j <= i + (keys - queries of the sequence).  A query
+ * row that sees no key, and every row of no sequence, gets 0 (lse -inf).  Query head h reads key /
+ * value head h / (hq / hkv).  Offsets are read on the device and clamped to the tensors.
+ * Rows may lie apart (*_row, *_head: strides in elements, the last dimension is dense); every row
+ * start must be 16-byte aligned.  out, out_low, dq, dk, dv are dense [rows, heads, d]. */
+typedef struct hv_attn_packed_args {
+  int dtype, hq, hkv, d;        /* HV_F32 / HV_BF16; hq % hkv == 0; d % 8 == 0, d <= 128 */
+  int nseq, causal;
+  float scale;                  /* > 0 */
+  int pad_;
+  long total_q, total_k;        /* rows of q / of k and v */
+  const int *cu_q, *cu_k;       /* [nseq + 1] device, ascending */
+  const void *q, *k, *v;
+  long q_row, q_head, k_row, k_head, v_row, v_head;
+  void* out;
+  void* out_low;                /* bf16 training: what out's rounding cut off, rounded to bf16 (NULL: not wanted) */
+  float* lse;                   /* [total_q, hq] log-sum-exp of the scaled scores (NULL: not wanted) */
+  void* work;                   /* forward / backward workspace of the size that the queries below give */
+  /* backward */
+  const void* dout;
+  long do_row, do_head;
+  void *dq, *dk, *dv;
+} hv_attn_packed_args;
+size_t hv_attn_packed_args_bytes(void);   /* sizeof, for bindings */
+size_t hv_attn_packed_work_bytes(const hv_attn_packed_args* a);
+int hv_attn_packed(const hv_attn_packed_args* a, hv_stream_t stream);
+/* dq, dk, dv from q, k, v, out (+ out_low), lse and dout; gradients of a shared key / value head are
+   summed over its query heads in fp32; rows of no sequence get 0.  No atomics. */
+size_t hv_attn_packed_backward_work_bytes(const hv_attn_packed_args* a);
+int hv_attn_packed_backward(const hv_attn_packed_args* a, hv_stream_t stream);
+
+/* s = x + residual;  y = s / sqrt(mean(s^2) + eps) * scale  (RMSNorm.forward,
+ * manifold_layers.py:449-456, after the residual addition of vit_encoder_decoder.py:190-208).
+ * x: x_dtype; residual (NULL: s = x, sum is not written) and sum: r_dtype; the sum is normalised
+ * before its rounding.  y_dtype HV_F32 / HV_BF16, or HV_E4M3 with y_scale [rows]: y ~ code * y_scale,
+ * y_scale = max(row's |y| / 448, 2^-120).  rstd [rows] (NULL: not wanted) = 1 / sqrt(mean + eps).
+ * All tensors dense [rows, cols]. */
+enum { HV_E4M3 = 3 /* OCP 8-bit float, 4 exponent and 3 mantissa bits */ };
+int hv_add_rmsnorm(int x_dtype, const void* x, int r_dtype, const void* residual, long rows, int cols, float eps,
+                   const float* scale, void* sum, int y_dtype, void* y, float* y_scale, float* rstd,
+                   hv_stream_t stream);
+/* dx (dx_dtype) and dresidual (r_dtype), the same values (either may be NULL), and dscale [cols] fp32 from the
+   stored sum, rstd, dy (dy_dtype) and dsum (r_dtype; NULL: the sum has no consumer).  No atomics. */
+size_t hv_add_rmsnorm_backward_work_floats(long rows, int cols);
+int hv_add_rmsnorm_backward(int r_dtype, const void* sum, const float* rstd, const float* scale, int dy_dtype,
+                            const void* dy, const void* dsum, long rows, int cols, int dx_dtype, void* dx,
+                            void* dresidual, float* dscale, float* work, hv_stream_t stream);
+
+/* rows of x (leading dimension ld) -> e4m3 codes, dense [rows, cols], and the scale of each row as above */
+int hv_quantize_rows_fp8(int dtype, const void* x, long ld, long rows, int cols, void* codes, float* scale,
+                         hv_stream_t stream);
+/* c[m, n] = act(a_scale[m] w_scale[n] sum_k a[m, k] w[n, k] + bias[n]): a, w e4m3 (nn.Linear, e.g. the MLP of
+   vit_encoder_decoder.py:146-152, on 8-bit rows); sums in fp32; c fp32 or bf16.  k, lda and ldw are multiples
+   of 16 and a, w 16-byte aligned.  work: hv_linear_fp8_work_bytes. */
+size_t hv_linear_fp8_work_bytes(long m, int n, int k);
+int hv_linear_fp8(const void* a, long lda, const float* a_scale, const void* w, long ldw, const float* w_scale,
+                  const float* bias, int act, long m, int n, int k, int c_dtype, void* c, long ldc, void* work,
+                  hv_stream_t stream);
 
 #ifdef __cplusplus
 }

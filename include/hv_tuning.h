@@ -28,6 +28,9 @@ enum hv_kernel_family {
   HV_KF_ATTN_GENERAL = 10,   /* hv_attention_general (cross / masked / weights / CLS-row queries) */
   HV_KF_GEMM_SMALLK = 11,    /* gemm_sk_kernel (persistent small-K, register epilogue) */
   HV_KF_GEMM_SPLITK = 12,    /* split-K LDS-DMA GEMM (64x64 tiles) + its reduce launch */
+  HV_KF_ATTN_PACKED = 13,    /* hv_attn_packed / hv_attn_packed_backward calls */
+  HV_KF_ADD_RMSNORM = 14,    /* hv_add_rmsnorm / hv_add_rmsnorm_backward calls */
+  HV_KF_LINEAR_FP8 = 15,     /* hv_linear_fp8 calls */
   HV_KF_COUNT = 16
 };
 /* copies the HV_KF_COUNT launch counters into out[] */

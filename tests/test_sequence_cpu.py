@@ -1,0 +1,137 @@
+"""CPU-side checks of the sequence operators: what the Python wrappers and the C entry points refuse, without a
+launch; shapes of the fake kernels."""
+import ctypes as C
+
+import pytest
+import torch
+
+
+@pytest.fixture
+def ops(monkeypatch):
+    """hv_amd.ops without its device check: every refusal below comes before a launch."""
+    from hv_amd import ops
+    monkeypatch.setattr(ops, "_cuda", lambda *t: None)
+    return ops
+
+
+def attn(ops, **kw):
+    a = dict(q=torch.zeros(6, 4, 32), k=torch.zeros(6, 2, 32), v=torch.zeros(6, 2, 32),
+             cu_q=torch.tensor([0, 6], dtype=torch.int32), cu_k=torch.tensor([0, 6], dtype=torch.int32))
+    extra = {n: kw.pop(n) for n in ("causal", "scale") if n in kw}
+    a.update(kw)
+    return ops.attn_packed_args(*a.values(), extra.get("causal", False), extra.get("scale"))
+
+
+def test_packed_attention_arguments(ops):
+    d = attn(ops, causal=True)
+    assert (d.hq, d.hkv, d.d, d.nseq, d.causal, d.total_q) == (4, 2, 32, 1, 1, 6)
+    assert abs(d.scale - 32 ** -0.5) < 1e-7
+    z = torch.zeros
+    bad = [dict(k=z(6, 3, 32), v=z(6, 3, 32)), dict(k=z(6, 2, 64)), dict(q=z(6, 128)), dict(k=z(6, 0, 32), v=z(6, 0, 32)),
+           dict(q=z(6, 4, 12), k=z(6, 2, 12), v=z(6, 2, 12)), dict(q=z(6, 4, 136), k=z(6, 2, 136), v=z(6, 2, 136)),
+           dict(k=z(6, 2, 32, dtype=torch.bfloat16)), dict(cu_q=torch.tensor([0, 6])),
+           dict(cu_k=torch.tensor([0, 3, 6], dtype=torch.int32)), dict(cu_q=z(0, dtype=torch.int32), cu_k=z(0, dtype=torch.int32)),
+           dict(q=z(6, 4, 33)[:, :, 1:]), dict(q=z(6, 4, 64)[:, :, ::2]), dict(scale=0.0), dict(scale=-1.0),
+           dict(scale=float("nan")), dict(scale=float("inf"))]
+    for kw in bad:
+        with pytest.raises(ValueError):
+            attn(ops, **kw)
+    with pytest.raises(TypeError):
+        attn(ops, q=z(6, 4, 32).double(), k=z(6, 2, 32).double(), v=z(6, 2, 32).double())
+
+
+def test_norm_and_linear_arguments(ops):
+    z, w = torch.zeros(4, 32), torch.ones(32)
+    for args in ((z, torch.zeros(4, 16), w), (z, torch.zeros(32), w), (z, z, torch.ones(16)), (z.t(), z.t(), torch.ones(4)),
+                 (torch.zeros(2, 0), torch.zeros(2, 0), torch.ones(0)), (torch.zeros(1, 32776), torch.zeros(1, 32776), torch.ones(32776))):
+        with pytest.raises(ValueError):
+            ops.add_rmsnorm(*args)
+        with pytest.raises(ValueError):
+            ops.add_rmsnorm_fp8(*args)
+    with pytest.raises(TypeError):
+        ops.add_rmsnorm(z, z, w.bfloat16())
+    with pytest.raises(ValueError):
+        ops.quantize_rows_fp8(torch.zeros(4))
+    with pytest.raises(ValueError):
+        ops.quantize_rows_fp8(torch.zeros(4, 8).t())
+    f8 = torch.float8_e4m3fn
+    a, b, s4, s3 = torch.zeros(4, 32).to(f8), torch.zeros(3, 32).to(f8), torch.ones(4), torch.ones(3)
+    for args, kw in (((z, s4, b, s3), {}), ((a, s3, b, s3), {}), ((a, s4, b, s4), {}), ((a, s4, b, s3), dict(bias=s4)),
+                     ((a, s4, b, s3), dict(act="tanh")), ((a[:, :24], s4, b[:, :24], s3), {}),
+                     ((torch.zeros(4, 48).to(f8)[:, 8:40], s4, b, s3), {}), ((a, s4.double(), b, s3), {}),
+                     ((torch.zeros(4, 16).to(f8), s4, b, s3), {})):
+        with pytest.raises(ValueError):
+            ops.linear_fp8(*args, **kw)
+    with pytest.raises(TypeError):
+        ops.linear_fp8(a, s4, b, s3, out_dtype=torch.float16)
+
+
+def test_product_path_refuses_cpu_tensors():
+    from hv_amd import ops
+    z = torch.zeros(4, 4, 32)
+    with pytest.raises(RuntimeError):
+        ops.attention_packed(z, z, z, torch.tensor([0, 4], dtype=torch.int32))
+    with pytest.raises(RuntimeError):
+        ops.add_rmsnorm(z, z, torch.ones(32))
+
+
+def test_c_entries_refuse():
+    """Argument errors of the C ABI come back as codes, nothing is launched."""
+    from hv_amd import _lib as L
+    lib = L.lib()
+    buf = torch.zeros(4096, dtype=torch.uint8)
+    p = (buf.data_ptr() + 63) // 64 * 64
+
+    def args(**kw):
+        a = L.AttnPackedArgs()
+        base = dict(dtype=1, hq=4, hkv=2, d=32, nseq=1, scale=0.5, total_q=4, total_k=4, cu_q=p, cu_k=p, q=p, k=p, v=p,
+                    q_row=128, q_head=32, k_row=64, k_head=32, v_row=64, v_head=32, out=p, lse=p, work=p, dout=p, do_row=128,
+                    do_head=32, dq=p, dk=p, dv=p)
+        base.update(kw)
+        for n, v in base.items():
+            setattr(a, n, v)
+        return C.byref(a)
+
+    inval = [dict(dtype=2), dict(hq=3), dict(hkv=0), dict(nseq=-1), dict(total_q=-1), dict(scale=0.0), dict(scale=-1.0),
+             dict(scale=float("nan")), dict(cu_q=None), dict(q=None), dict(k=p + 2), dict(v_row=61), dict(q_head=3)]
+    for kw in inval:
+        assert lib.hv_attn_packed(args(**kw), None) == -1, kw
+        assert lib.hv_attn_packed_backward(args(**kw), None) == -1, kw
+    for kw in (dict(d=12), dict(d=136), dict(d=0), dict(total_q=1 << 30), dict(total_k=1 << 30)):
+        assert lib.hv_attn_packed(args(**kw), None) == -2, kw
+    assert lib.hv_attn_packed(args(out=None), None) == -1
+    assert lib.hv_attn_packed(None, None) == -1
+    for kw in (dict(dout=None), dict(lse=None), dict(work=None), dict(dk=None), dict(dv=p + 8), dict(dq=p + 8)):
+        assert lib.hv_attn_packed_backward(args(**kw), None) == -1, kw
+    assert lib.hv_attn_packed(args(total_q=0), None) == 0                   # nothing to do
+    assert lib.hv_add_rmsnorm(0, p, 0, p, 0, 32, 1e-8, p, p, 0, p, None, None, None) == 0
+    for bad in ((5, p, 0, p, 2, 32, 1e-8, p, p, 0, p, None, None), (0, p, 0, p, 2, 0, 1e-8, p, p, 0, p, None, None),
+                (0, p, 0, p, 2, 32, -1.0, p, p, 0, p, None, None), (0, None, 0, p, 2, 32, 1e-8, p, p, 0, p, None, None),
+                (0, p, 0, p, 2, 32, 1e-8, p, None, 0, p, None, None), (0, p, 0, p, 2, 32, 1e-8, p, p, 3, p, None, None),
+                (0, p, 0, p, 2, 32, 1e-8, p, p, 2, p, None, None)):
+        assert lib.hv_add_rmsnorm(*bad, None) == -1, bad
+    assert lib.hv_add_rmsnorm(0, p, 0, p, 2, 32769, 1e-8, p, p, 0, p, None, None, None) == -2
+    assert lib.hv_add_rmsnorm_backward(0, p, p, p, 0, None, p, 2, 32, 0, p, p, p, p, None) == -1
+    assert lib.hv_quantize_rows_fp8(0, p, 16, 2, 32, p, p, None) == -1
+    for bad, rc in (((p, 32, p, p, 32, p, None, 9, 4, 4, 32, 1, p, 4, None), -1), ((p, 32, p, p, 32, p, None, 0, 4, 4, 32, 2, p, 4, None), -1),
+                    ((p, 16, p, p, 32, p, None, 0, 4, 4, 32, 1, p, 4, None), -1), ((p, 32, p, p, 32, p, None, 0, 4, 4, 24, 1, p, 4, None), -2),
+                    ((p + 1, 32, p, p, 32, p, None, 0, 4, 4, 32, 1, p, 4, None), -1), ((p, 32, None, p, 32, p, None, 0, 4, 4, 32, 1, p, 4, None), -1)):
+        assert lib.hv_linear_fp8(*bad, None) == rc, bad
+
+
+def test_fake_kernels():
+    import hv_amd  # noqa: F401
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        d = "cuda"
+        q, k = torch.empty(10, 4, 64, device=d, dtype=torch.bfloat16), torch.empty(12, 2, 64, device=d, dtype=torch.bfloat16)
+        cu = torch.empty(3, device=d, dtype=torch.int32)
+        out, lse = torch.ops.hv.attention_packed(q, k, k, cu, cu, True)
+        assert out.shape == q.shape and lse.shape == (10, 4) and lse.dtype == torch.float32
+        x, r, w = torch.empty(5, 64, device=d, dtype=torch.bfloat16), torch.empty(5, 64, device=d), torch.empty(64, device=d)
+        y, s = torch.ops.hv.add_rmsnorm(x, r, w)
+        assert y.dtype == torch.bfloat16 and s.dtype == torch.float32
+        c, sc, s = torch.ops.hv.add_rmsnorm_fp8(x, r, w)
+        assert c.dtype == torch.float8_e4m3fn and sc.shape == (5,)
+        w8, ws = torch.ops.hv.quantize_rows_fp8(torch.empty(7, 64, device=d))
+        assert torch.ops.hv.linear_fp8(c, sc, w8, ws).shape == (5, 7)
