@@ -181,6 +181,17 @@ __device__ __forceinline__ Tile find_tile(const int* __restrict__ cu, int nseq, 
   return t;
 }
 
+// the sequence that owns row `row` (nseq: none)
+__device__ __forceinline__ int find_row(const int* __restrict__ cu, int nseq, long total, int row) {
+  for (int s0 = 0; s0 < nseq; s0 += 64) {
+    const int s = s0 + (threadIdx.x & 63);
+    const bool in = s < nseq && clamp_row(cu[s], (int)total) <= row && row < clamp_row(cu[s + 1], (int)total);
+    const unsigned long long hit = __ballot(in);
+    if (hit) return s0 + __builtin_ctzll(hit);
+  }
+  return nseq;
+}
+
 // rows of sequence `seq` on the other side (none for the two outside ranges)
 __device__ __forceinline__ void seq_rows(const int* __restrict__ cu, int nseq, long total, int seq, int& start, int& len) {
   if (seq >= nseq) { start = len = 0; return; }
@@ -212,6 +223,13 @@ template <typename T, int DP, int ROWS> struct Stage {
     }
   }
 };
+
+__device__ __forceinline__ void load8(Frag<unsigned short>& f, const unsigned short* p) { f.v = *(const bf16x8*)p; }
+__device__ __forceinline__ void load8(Frag<float>& f, const float* p) {
+  const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) { f.v[e] = a[e]; f.v[4 + e] = b[e]; }
+}
 
 // a lane's row of 16-column operands straight from memory (null: zeros)
 template <typename T, int DP> __device__ __forceinline__ void load_row(Frag<T>* f, const T* p, int d, int h) {
@@ -396,23 +414,229 @@ __global__ void __launch_bounds__(NT) k_attn_packed(const hv_attn_packed_args a)
 }
 
 // ------------------------------------------------------------------------------------------------
-// delta_i = dO_i . O_i = sum_j P_ij dP_ij (the mean that the softmax gradient subtracts): one wave per row
+// Forward with few query rows (new tokens against histories): the keys are cut into parts of a.part and a block
+// takes one part for all the rows of its sequence, 32 at a time.  Its four waves own a quarter of the part each, in
+// slabs of 32 keys, and never wait for one another: K goes from memory to registers as the first operand, V through a
+// wave's own LDS, both a slab ahead, so a wave has 2 * 32 rows in flight and a CU eight such waves.  Bytes bound it.
+// Partial sums (fp32, with their maxima) go to the workspace and are joined by k_attn_packed_join in a fixed order.
+template <typename T, int DP>
+__global__ void __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) k_attn_packed_keys(const hv_attn_packed_args a, int part_keys, float* __restrict__ po,
+                                                         float4* __restrict__ pml) {
+  using L = Lay<T, DP>;
+  constexpr int SB = 32 * L::ROWB;                       // a wave's V slab
+  constexpr int JB = 32 * DP * 4;                        // a wave's O at the end, fp32
+  constexpr int NV = 32 * L::CH / 64;                    // its 16-byte chunks per lane
+  __shared__ __align__(16) char smem[4 * SB > 2 * JB ? 4 * SB : 2 * JB];
+  __shared__ float red[3][4][32];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, c31 = lane & 31;
+  const int kvh = blockIdx.x % a.hkv, G = a.hq / a.hkv;
+  const Tile t = find_tile(a.cu_k, a.nseq, a.total_k, 1, part_keys, blockIdx.x / a.hkv, false);
+  if (t.seq < 0 || t.seq >= a.nseq) return;
+  int q0, lq;
+  seq_rows(a.cu_q, a.nseq, a.total_q, t.seq, q0, lq);
+  const int lk = t.len, late = lk - lq, quarter = part_keys >> 2;
+  const int key0 = t.tile * part_keys + wave * quarter, key1 = min(key0 + quarter, lk);
+  const T* kp = (const T*)a.k + (long)t.start * a.k_row + (long)kvh * a.k_head;
+  const T* vp = (const T*)a.v + (long)t.start * a.v_row + (long)kvh * a.v_head;
+  const float c2 = a.scale * LOG2E;
+  const View<T, DP> view(lane);
+  char* slab = smem + wave * SB;
+  for (long r0 = 0; r0 < (long)lq * G; r0 += 32) {
+    const long r = r0 + c31;
+    const bool real = r < (long)lq * G;
+    const int tok = real ? (int)(r / G) : 0, qh = kvh * G + (int)(r % G);
+    const long qrow = (long)q0 + tok;
+    const int lim = !real ? -1 : (a.causal ? min(tok + late, lk - 1) : lk - 1);
+    Frag<T> q[L::NS], k[L::NS];
+    load_row<T, DP>(q, real ? (const T*)a.q + qrow * a.q_row + (long)qh * a.q_head : nullptr, a.d, h);
+    u32x4 v[NV];
+    auto fetch = [&](int key) {
+      load_row<T, DP>(k, key + c31 < key1 ? kp + (long)(key + c31) * a.k_row : nullptr, a.d, h);
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        const int i = lane + n * 64, row = i / L::CH, c = i % L::CH;
+        v[n] = key + row < key1 && c * L::EPC < a.d ? *(const u32x4*)(vp + (long)(key + row) * a.v_row + c * L::EPC)
+                                                    : u32x4{0, 0, 0, 0};
+      }
+    };
+    f32x16 o[L::NDT];
+#pragma unroll
+    for (int i = 0; i < L::NDT; ++i) o[i] = zero16();
+    float m = NEG_INF, l = 0.f, lt = 0.f;                // maximum, sums of the rounded / the exact weights
+    if (key0 < key1) fetch(key0);
+    for (int key = key0; key < key1; key += 32) {
+      f32x16 s = zero16();
+#pragma unroll
+      for (int i = 0; i < L::NS; ++i) s = mma16(k[i], q[i], s);
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        const int i = lane + n * 64, row = i / L::CH, c = i % L::CH;
+        *(u32x4*)(slab + row * L::ROWB + ((c ^ L::f(row)) << 4)) = v[n];
+      }
+      __builtin_amdgcn_wave_barrier();
+      if (key + 32 < key1) fetch(key + 32);
+      const int last = min(lim, key1 - 1);
+      if (__any(key + 31 > last)) {
+#pragma unroll
+        for (int x = 0; x < 16; ++x)
+          if (key + 8 * (x >> 2) + 4 * h + (x & 3) > last) s[x] = NEG_INF;
+      }
+      float top = s[0];
+#pragma unroll
+      for (int x = 1; x < 16; ++x) top = fmaxf(top, s[x]);
+      top = fmaxf(top, other_half(top));
+      if (__any((top - m) * c2 > 8.f)) {
+        const float mn = fmaxf(m, top);
+        const float alpha = mn == NEG_INF ? 1.f : __builtin_amdgcn_exp2f((m - mn) * c2);
+        m = mn;
+        l *= alpha;
+        lt *= alpha;
+#pragma unroll
+        for (int i = 0; i < L::NDT; ++i)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) o[i][x] *= alpha;
+      }
+      const float mc = m == NEG_INF ? 0.f : -m * c2;
+#pragma unroll
+      for (int x = 0; x < 16; ++x) s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], c2, mc));
+      if (a.lse) {
+#pragma unroll
+        for (int x = 0; x < 16; ++x) lt += s[x];
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const Frag<T> p = from_acc<T>(s, i);
+        l = add_sum(p, l);
+#pragma unroll
+        for (int dt = 0; dt < L::NDT; ++dt) o[dt] = mma16(view.cols(slab + 16 * i * L::ROWB, dt), p, o[dt]);
+      }
+    }
+    l += other_half(l);
+    lt += other_half(lt);
+    // the four quarters of the part: common maximum, then the sums in the order 0 + 2, 1 + 3, (0 2) + (1 3)
+    __syncthreads();
+    if (h == 0) { red[0][wave][c31] = m; red[1][wave][c31] = l; red[2][wave][c31] = lt; }
+    __syncthreads();
+    float mx = NEG_INF, lsum = 0.f, ltsum = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mx = fmaxf(mx, red[0][w][c31]);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float mw = red[0][w][c31], f = mw == NEG_INF ? 1.f : __builtin_amdgcn_exp2f((mw - mx) * c2);
+      lsum = fmaf(red[1][w][c31], f, lsum);
+      ltsum = fmaf(red[2][w][c31], f, ltsum);
+    }
+    const float f = m == NEG_INF ? 1.f : __builtin_amdgcn_exp2f((m - mx) * c2);
+#pragma unroll
+    for (int i = 0; i < L::NDT; ++i)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) o[i][x] *= f;
+    float* mine = (float*)(smem + (wave & 1) * JB);
+#pragma unroll
+    for (int step = 2; step > 0; step >>= 1) {
+      if (wave >= step && wave < 2 * step) {
+#pragma unroll
+        for (int i = 0; i < L::NDT; ++i)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) ((step == 1 ? (float*)smem : mine))[(i * 16 + x) * 64 + lane] = o[i][x];
+      }
+      __syncthreads();
+      if (wave < step) {
+#pragma unroll
+        for (int i = 0; i < L::NDT; ++i)
+#pragma unroll
+          for (int x = 0; x < 16; ++x) o[i][x] += ((step == 1 ? (float*)smem : mine))[(i * 16 + x) * 64 + lane];
+      }
+      __syncthreads();
+    }
+    if (wave == 0 && real) {
+      const long at = ((long)t.tile * a.total_q + qrow) * a.hq + qh;
+      store_row<float, DP>(po + at * a.d, a.d, h, o, 1.f);
+      if (h == 0) pml[at] = make_float4(mx, lsum, ltsum, 0.f);
+    }
+  }
+}
+
+// out and lse from the parts: one wave per (token, head)
+template <typename T>
+__global__ void __launch_bounds__(NT) k_attn_packed_join(const hv_attn_packed_args a, int part_keys,
+                                                         const float* __restrict__ po, const float4* __restrict__ pml) {
+  const long i = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (i >= a.total_q * a.hq) return;
+  const int lane = threadIdx.x & 63;
+  int k0, lk;
+  seq_rows(a.cu_k, a.nseq, a.total_k, find_row(a.cu_q, a.nseq, a.total_q, (int)(i / a.hq)), k0, lk);
+  const int parts = (lk + part_keys - 1) / part_keys;
+  const long step = a.total_q * a.hq;
+  const float c2 = a.scale * LOG2E;
+  float m = NEG_INF, l = 0.f, lt = 0.f, acc[2] = {0.f, 0.f};
+  const bool in0 = lane < a.d, in1 = lane + 64 < a.d;
+  for (int z0 = 0; z0 < parts; z0 += 64) {               // 64 parts at a time: a lane holds one part's maximum and sums
+    const int n = min(64, parts - z0);
+    const float4 ml = lane < n ? pml[(z0 + lane) * step + i] : make_float4(NEG_INF, 0.f, 0.f, 0.f);
+    const float mn = fmaxf(m, wave_max(ml.x));
+    const float old = m == NEG_INF ? 1.f : __builtin_amdgcn_exp2f((m - mn) * c2);
+    const float w = ml.x == NEG_INF ? (ml.y == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f((ml.x - mn) * c2);
+    m = mn;
+    l = l * old + wave_sum(ml.y * w);
+    lt = lt * old + wave_sum(ml.z * w);
+    acc[0] *= old;
+    acc[1] *= old;
+    const float* p = po + (z0 * step + i) * a.d + lane;
+    int z = 0;
+    for (; z + 4 <= n; z += 4) {                         // four parts' loads in flight
+      float x[4], y[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[j] = in0 ? p[(z + j) * step * a.d] : 0.f;
+        y[j] = in1 ? p[(z + j) * step * a.d + 64] : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float wz = __shfl(w, z + j, 64);
+        acc[0] = fmaf(x[j], wz, acc[0]);
+        acc[1] = fmaf(y[j], wz, acc[1]);
+      }
+    }
+    for (; z < n; ++z) {
+      const float wz = __shfl(w, z, 64);
+      if (in0) acc[0] = fmaf(p[z * step * a.d], wz, acc[0]);
+      if (in1) acc[1] = fmaf(p[z * step * a.d + 64], wz, acc[1]);
+    }
+  }
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    if (lane + 64 * e < a.d) {
+      const float v = acc[e] * inv;
+      Elem<T>::store((T*)a.out + i * a.d, lane + 64 * e, v);
+      if constexpr (sizeof(T) == 2)
+        if (a.out_low) Elem<T>::store((T*)a.out_low + i * a.d, lane + 64 * e, v - bf2f(f2bf(v)));
+    }
+  if (a.lse && lane == 0) a.lse[i] = lt > 0.f || lt != lt ? m * a.scale + __logf(lt) : NEG_INF;
+}
+
+// ------------------------------------------------------------------------------------------------
+// delta_i = dO_i . O_i = sum_j P_ij dP_ij (the mean that the softmax gradient subtracts): 16 lanes per row
 template <typename T>
 __global__ void __launch_bounds__(NT) k_attn_packed_delta(const hv_attn_packed_args a, float* __restrict__ delta) {
-  const int lane = threadIdx.x & 63;
-  for (long i = (long)blockIdx.x * 4 + (threadIdx.x >> 6); i < a.total_q * a.hq; i += (long)gridDim.x * 4) {
-    const long row = i / a.hq;
-    const T* po = (const T*)a.out + i * a.d;
-    const T* pl = (const T*)a.out_low;
-    const T* pd = (const T*)a.dout + row * a.do_row + (i % a.hq) * a.do_head;
+  const int c = (threadIdx.x & 15) * 8;                  // d <= 128
+  const long rows = a.total_q * a.hq;
+  for (long i = (long)blockIdx.x * 16 + (threadIdx.x >> 4); i < rows; i += (long)gridDim.x * 16) {
     float s = 0.f;
-    for (int c = lane; c < a.d; c += 64) {
-      float v = Elem<T>::load(po, c);
-      if (pl) v += Elem<T>::load(pl + i * a.d, c);
-      s = fmaf(v, Elem<T>::load(pd, c), s);
+    if (c < a.d) {
+      Frag<T> o, g, low;
+      const T* pg = (const T*)a.dout + (i / a.hq) * a.do_row + (i % a.hq) * a.do_head + c;
+      load8(o, (const T*)a.out + i * a.d + c);
+      load8(g, pg);
+      if (a.out_low) load8(low, (const T*)a.out_low + i * a.d + c);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s = fmaf((float)o.v[e] + (a.out_low ? (float)low.v[e] : 0.f), (float)g.v[e], s);
     }
-    s = wave_sum(s);
-    if (lane == 0) delta[i] = s;
+#pragma unroll
+    for (int x = 8; x > 0; x >>= 1) s += __shfl_xor(s, x, 64);
+    if (c == 0) delta[i] = s;
   }
 }
 
@@ -620,12 +844,19 @@ bool aligned(const void* p, long row, long head, int es) {
   return p != nullptr && ((uintptr_t)p & 15) == 0 && (row * es) % 16 == 0 && (head * es) % 16 == 0 && row >= 0 && head >= 0;
 }
 
-int check_args(const hv_attn_packed_args* a) {
+int check_shape(const hv_attn_packed_args* a) {
   if (a == nullptr || (a->dtype != HV_F32 && a->dtype != HV_BF16)) return HV_EINVAL;
   if (a->hq <= 0 || a->hkv <= 0 || a->hq % a->hkv || a->nseq < 0 || a->total_q < 0 || a->total_k < 0) return HV_EINVAL;
-  if (!(a->scale > 0.f) || a->scale > 3.0e38f || a->cu_q == nullptr || a->cu_k == nullptr) return HV_EINVAL;
+  if (!(a->scale > 0.f) || a->scale > 3.0e38f) return HV_EINVAL;
   if (a->d <= 0 || a->d % 8 || a->d > 128 || a->hq > 1024) return HV_EUNSUPPORTED;
   if (a->total_q >= (1L << 30) || a->total_k >= (1L << 30)) return HV_EUNSUPPORTED;
+  return HV_OK;
+}
+
+int check_args(const hv_attn_packed_args* a) {
+  const int rc = check_shape(a);
+  if (rc != HV_OK) return rc;
+  if (a->cu_q == nullptr || a->cu_k == nullptr) return HV_EINVAL;
   const int es = a->dtype == HV_BF16 ? 2 : 4;
   if (a->total_q && (!aligned(a->q, a->q_row, a->q_head, es))) return HV_EINVAL;
   if (a->total_k && (!aligned(a->k, a->k_row, a->k_head, es) || !aligned(a->v, a->v_row, a->v_head, es))) return HV_EINVAL;
@@ -637,6 +868,27 @@ constexpr long MAX_BLOCKS = 1L << 24;                    // a grid stays below 2
 // blocks that cover `total` rows in nseq sequences and the two ranges outside of them, BM packed rows each
 long tile_bound(long total, int nseq, int G, int BM) { return total * G / BM + nseq + 2; }
 
+// Keys of a part in the few-rows form, 0: the tile form.  Few rows: on average at most 64 packed rows per sequence (the
+// tile form would leave its second tile half empty and give one block all of a sequence's keys).  Parts are sized for
+// about four blocks per CU, 128 keys (one slab per wave) at least.
+int part_keys(const hv_attn_packed_args& a) {
+  const int G = a.hq / a.hkv;
+  if (a.nseq == 0 || a.total_q == 0 || a.total_k == 0 || a.total_q * G > 64L * a.nseq) return 0;
+  long n = (a.total_k * a.hkv + 1023) / 1024;
+  n = (n + 127) / 128 * 128;
+  return (int)(n < 128 ? 128 : n);
+}
+size_t part_rows(const hv_attn_packed_args& a, int n) { return (size_t)((a.total_k + n - 1) / n) * a.total_q * a.hq; }
+
+template <typename T, int DP> void launch_keys(const hv_attn_packed_args& a, int n, hipStream_t s) {
+  const size_t rows = part_rows(a, n);
+  float* po = (float*)a.work;
+  float4* pml = (float4*)(po + rows * a.d);
+  const unsigned blocks = (unsigned)(tile_bound(a.total_k, a.nseq, 1, n) * a.hkv);
+  k_attn_packed_keys<T, DP><<<blocks, NT, 0, s>>>(a, n, po, pml);
+  k_attn_packed_join<T><<<hv_cdiv(a.total_q * a.hq, 4), NT, 0, s>>>(a, n, po, pml);
+}
+
 template <typename T, int DP> void launch_forward(const hv_attn_packed_args& a, unsigned blocks, hipStream_t s) {
   if (a.lse != nullptr || a.out_low != nullptr) k_attn_packed<T, DP, true><<<blocks, NT, 0, s>>>(a);
   else k_attn_packed<T, DP, false><<<blocks, NT, 0, s>>>(a);
@@ -645,7 +897,7 @@ template <typename T, int DP> void launch_forward(const hv_attn_packed_args& a, 
 template <typename T, int DP>
 void launch_backward(const hv_attn_packed_args& a, unsigned bq, unsigned bk, float* delta, hipStream_t s) {
   if (a.total_q) {
-    k_attn_packed_delta<T><<<(unsigned)min((a.total_q * a.hq + 3) / 4, 1L << 20), NT, 0, s>>>(a, delta);
+    k_attn_packed_delta<T><<<(unsigned)min((a.total_q * a.hq + 15) / 16, 1L << 20), NT, 0, s>>>(a, delta);
     if (a.dq) k_attn_packed_dq<T, DP><<<bq, NT, 0, s>>>(a, delta);
   }
   if (a.total_k && a.dk) k_attn_packed_dkv<T, DP><<<bk, NT, 0, s>>>(a, delta);
@@ -663,7 +915,11 @@ void launch_backward(const hv_attn_packed_args& a, unsigned bq, unsigned bk, flo
 
 extern "C" size_t hv_attn_packed_args_bytes(void) { return sizeof(hv_attn_packed_args); }
 
-extern "C" size_t hv_attn_packed_work_bytes(const hv_attn_packed_args*) { return 0; }
+extern "C" size_t hv_attn_packed_work_bytes(const hv_attn_packed_args* a) {
+  if (check_shape(a) != HV_OK) return 0;
+  const int n = part_keys(*a);
+  return n ? part_rows(*a, n) * (a->d + 4) * sizeof(float) : 0;
+}
 
 extern "C" int hv_attn_packed(const hv_attn_packed_args* a, hv_stream_t stream) {
   const int rc = check_args(a);
@@ -673,7 +929,13 @@ extern "C" int hv_attn_packed(const hv_attn_packed_args* a, hv_stream_t stream) 
   const long blocks = tile_bound(a->total_q, a->nseq, a->hq / a->hkv, 128) * a->hkv;
   if (blocks >= MAX_BLOCKS) return HV_EUNSUPPORTED;
   hipStream_t s = (hipStream_t)stream;
-  HV_DISPATCH(a->dtype, HV_HEAD_DIM(a->d, launch_forward, *a, (unsigned)blocks, s));
+  const int n = part_keys(*a);
+  if (n) {
+    if (a->work == nullptr || ((uintptr_t)a->work & 15) || tile_bound(a->total_k, a->nseq, 1, n) * a->hkv >= MAX_BLOCKS)
+      return HV_EINVAL;
+    HV_DISPATCH(a->dtype, HV_HEAD_DIM(a->d, launch_keys, *a, n, s));
+  } else
+    HV_DISPATCH(a->dtype, HV_HEAD_DIM(a->d, launch_forward, *a, (unsigned)blocks, s));
   HV_CHECK_LAUNCH();
   hv_diag_count(HV_KF_ATTN_PACKED);
   return HV_OK;
@@ -687,7 +949,8 @@ extern "C" int hv_attn_packed_backward(const hv_attn_packed_args* a, hv_stream_t
   const int rc = check_args(a);
   if (rc != HV_OK) return rc;
   const int es = a->dtype == HV_BF16 ? 2 : 4;
-  if (a->total_q && (!aligned(a->dout, a->do_row, a->do_head, es) || a->out == nullptr || a->lse == nullptr ||
+  if (a->total_q && (!aligned(a->dout, a->do_row, a->do_head, es) || !aligned(a->out, 0, 0, es) ||
+                     ((uintptr_t)a->out_low & 15) || a->lse == nullptr ||
                      ((uintptr_t)a->dq & 15) || a->work == nullptr))
     return HV_EINVAL;
   if ((a->dk == nullptr) != (a->dv == nullptr) || ((uintptr_t)a->dk & 15) || ((uintptr_t)a->dv & 15)) return HV_EINVAL;
