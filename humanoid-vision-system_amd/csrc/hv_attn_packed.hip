@@ -24,6 +24,23 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
+// division by a number fixed on the host: x / d for 0 <= x < 2^31 is (mulhi(x, mul) + x) >> shift
+struct FastDiv {
+  uint32_t mul, shift, d;
+  explicit FastDiv(uint32_t v) : shift(0), d(v) {
+    while ((1ull << shift) < v) ++shift;
+    mul = (uint32_t)((((1ull << 32) * ((1ull << shift) - v)) / v) + 1);
+  }
+  __device__ __forceinline__ int div(int x) const { return (int)((__umulhi((uint32_t)x, mul) + (uint32_t)x) >> shift); }
+  __device__ __forceinline__ int mod(int x, int q) const { return x - q * (int)d; }
+};
+
+// what the kernels get: the call's arguments, the query heads per key / value head and the key / value heads
+struct Args : hv_attn_packed_args {
+  FastDiv group, heads;
+  explicit Args(const hv_attn_packed_args& a) : hv_attn_packed_args(a), group(a.hq / a.hkv), heads(a.hkv) {}
+};
+
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int NT = 256;         // threads of every block: 4 waves
 constexpr float NEG_INF = -__builtin_inff();
@@ -280,25 +297,25 @@ __device__ __forceinline__ f32x16 zero16() {
 // ------------------------------------------------------------------------------------------------
 // Forward: 4 waves of 32 packed rows each over tiles of BN keys that the block stages once.
 template <typename T, int DP, bool TRAIN>
-__global__ void __launch_bounds__(NT) k_attn_packed(const hv_attn_packed_args a) {
+__global__ void __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) k_attn_packed(const Args a) {
   using L = Lay<T, DP>;
   constexpr int BM = 128, BN = 64, TB = BN * L::ROWB;
   __shared__ __align__(16) char smem[2 * TB];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-  const int kvh = blockIdx.x % a.hkv, G = a.hq / a.hkv;
-  const Tile t = find_tile(a.cu_q, a.nseq, a.total_q, G, BM, blockIdx.x / a.hkv, a.causal != 0);
+  const int G = a.group.d, block = a.heads.div(blockIdx.x), kvh = a.heads.mod(blockIdx.x, block);
+  const Tile t = find_tile(a.cu_q, a.nseq, a.total_q, G, BM, block, a.causal != 0);
   if (t.seq < 0) return;
   int k0, lk;
   seq_rows(a.cu_k, a.nseq, a.total_k, t.seq, k0, lk);
 
-  const long r = (long)t.tile * BM + wave * 32 + (lane & 31);
-  const bool real = r < (long)t.len * G;
-  const int tok = real ? (int)(r / G) : 0, g = (int)(r % G);
+  const int r = t.tile * BM + wave * 32 + (lane & 31);
+  const bool real = r < t.len * G;
+  const int tok = real ? a.group.div(r) : 0, g = real ? a.group.mod(r, tok) : 0;
   const int late = lk - t.len;                           // the last query sees every key
   const int lim = !real ? -1 : (a.causal ? min(tok + late, lk - 1) : lk - 1);     // last key of this row
   // the block's last key, the wave's first row's last key: full tiles need no mask
-  const long last_r = min((long)(t.tile + 1) * BM, (long)t.len * G) - 1;
-  const int lim_blk = a.causal ? min((int)(last_r / G) + late, lk - 1) : lk - 1;
+  const int last_r = min((t.tile + 1) * BM, t.len * G) - 1;
+  const int lim_blk = a.causal ? min(a.group.div(last_r) + late, lk - 1) : lk - 1;
   int lim_lo = lim, lim_hi = lim;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -420,7 +437,7 @@ __global__ void __launch_bounds__(NT) k_attn_packed(const hv_attn_packed_args a)
 // wave's own LDS, both a slab ahead, so a wave has 2 * 32 rows in flight and a CU eight such waves.  Bytes bound it.
 // Partial sums (fp32, with their maxima) go to the workspace and are joined by k_attn_packed_join in a fixed order.
 template <typename T, int DP>
-__global__ void __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) k_attn_packed_keys(const hv_attn_packed_args a, int part_keys, float* __restrict__ po,
+__global__ void __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) k_attn_packed_keys(const Args a, int part_keys, float* __restrict__ po,
                                                          float4* __restrict__ pml) {
   using L = Lay<T, DP>;
   constexpr int SB = 32 * L::ROWB;                       // a wave's V slab
@@ -429,8 +446,8 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) k_att
   __shared__ __align__(16) char smem[4 * SB > 2 * JB ? 4 * SB : 2 * JB];
   __shared__ float red[3][4][32];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, c31 = lane & 31;
-  const int kvh = blockIdx.x % a.hkv, G = a.hq / a.hkv;
-  const Tile t = find_tile(a.cu_k, a.nseq, a.total_k, 1, part_keys, blockIdx.x / a.hkv, false);
+  const int G = a.group.d, block = a.heads.div(blockIdx.x), kvh = a.heads.mod(blockIdx.x, block);
+  const Tile t = find_tile(a.cu_k, a.nseq, a.total_k, 1, part_keys, block, false);
   if (t.seq < 0 || t.seq >= a.nseq) return;
   int q0, lq;
   seq_rows(a.cu_q, a.nseq, a.total_q, t.seq, q0, lq);
@@ -441,10 +458,10 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) k_att
   const float c2 = a.scale * LOG2E;
   const View<T, DP> view(lane);
   char* slab = smem + wave * SB;
-  for (long r0 = 0; r0 < (long)lq * G; r0 += 32) {
-    const long r = r0 + c31;
-    const bool real = r < (long)lq * G;
-    const int tok = real ? (int)(r / G) : 0, qh = kvh * G + (int)(r % G);
+  for (int r0 = 0; r0 < lq * G; r0 += 32) {
+    const int r = r0 + c31;
+    const bool real = r < lq * G;
+    const int tok = real ? a.group.div(r) : 0, qh = kvh * G + (real ? a.group.mod(r, tok) : 0);
     const long qrow = (long)q0 + tok;
     const int lim = !real ? -1 : (a.causal ? min(tok + late, lk - 1) : lk - 1);
     Frag<T> q[L::NS], k[L::NS];
@@ -560,7 +577,7 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) k_att
 
 // out and lse from the parts: one wave per (token, head)
 template <typename T>
-__global__ void __launch_bounds__(NT) k_attn_packed_join(const hv_attn_packed_args a, int part_keys,
+__global__ void __launch_bounds__(NT) k_attn_packed_join(const Args a, int part_keys,
                                                          const float* __restrict__ po, const float4* __restrict__ pml) {
   const long i = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (i >= a.total_q * a.hq) return;
@@ -620,7 +637,7 @@ __global__ void __launch_bounds__(NT) k_attn_packed_join(const hv_attn_packed_ar
 // ------------------------------------------------------------------------------------------------
 // delta_i = dO_i . O_i = sum_j P_ij dP_ij (the mean that the softmax gradient subtracts): 16 lanes per row
 template <typename T>
-__global__ void __launch_bounds__(NT) k_attn_packed_delta(const hv_attn_packed_args a, float* __restrict__ delta) {
+__global__ void __launch_bounds__(NT) k_attn_packed_delta(const Args a, float* __restrict__ delta) {
   const int c = (threadIdx.x & 15) * 8;                  // d <= 128
   const long rows = a.total_q * a.hq;
   for (long i = (long)blockIdx.x * 16 + (threadIdx.x >> 4); i < rows; i += (long)gridDim.x * 16) {
@@ -642,23 +659,23 @@ __global__ void __launch_bounds__(NT) k_attn_packed_delta(const hv_attn_packed_a
 
 // dQ: the forward's walk over the keys with dO beside Q; dQ^T += K^T dS^T
 template <typename T, int DP>
-__global__ void __launch_bounds__(NT) k_attn_packed_dq(const hv_attn_packed_args a, const float* __restrict__ delta) {
+__global__ void __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) k_attn_packed_dq(const Args a, const float* __restrict__ delta) {
   using L = Lay<T, DP>;
   constexpr int BM = 128, BN = 64, TB = BN * L::ROWB;
   __shared__ __align__(16) char smem[2 * TB];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-  const int kvh = blockIdx.x % a.hkv, G = a.hq / a.hkv;
-  const Tile t = find_tile(a.cu_q, a.nseq, a.total_q, G, BM, blockIdx.x / a.hkv, a.causal != 0);
+  const int G = a.group.d, block = a.heads.div(blockIdx.x), kvh = a.heads.mod(blockIdx.x, block);
+  const Tile t = find_tile(a.cu_q, a.nseq, a.total_q, G, BM, block, a.causal != 0);
   if (t.seq < 0) return;
   int k0, lk;
   seq_rows(a.cu_k, a.nseq, a.total_k, t.seq, k0, lk);
-  const long r = (long)t.tile * BM + wave * 32 + (lane & 31);
-  const bool real = r < (long)t.len * G;
-  const int tok = real ? (int)(r / G) : 0, g = (int)(r % G);
+  const int r = t.tile * BM + wave * 32 + (lane & 31);
+  const bool real = r < t.len * G;
+  const int tok = real ? a.group.div(r) : 0, g = real ? a.group.mod(r, tok) : 0;
   const int late = lk - t.len;
   const int lim = !real ? -1 : (a.causal ? min(tok + late, lk - 1) : lk - 1);
-  const long last_r = min((long)(t.tile + 1) * BM, (long)t.len * G) - 1;
-  const int lim_blk = a.causal ? min((int)(last_r / G) + late, lk - 1) : lk - 1;
+  const int last_r = min((t.tile + 1) * BM, t.len * G) - 1;
+  const int lim_blk = a.causal ? min(a.group.div(last_r) + late, lk - 1) : lk - 1;
   int lim_lo = lim, lim_hi = lim;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -727,14 +744,14 @@ __global__ void __launch_bounds__(NT) k_attn_packed_dq(const hv_attn_packed_args
 
 // dK, dV: a wave holds 32 keys and walks over the packed rows of its sequence (all heads of the group)
 template <typename T, int DP>
-__global__ void __launch_bounds__(NT, 1) k_attn_packed_dkv(const hv_attn_packed_args a, const float* __restrict__ delta) {
+__global__ void __launch_bounds__(NT, DP == 128 || sizeof(T) == 4 ? 1 : 2) k_attn_packed_dkv(const Args a, const float* __restrict__ delta) {
   using L = Lay<T, DP>;
   constexpr int BK = 128, BR = L::ROWB >= 512 ? 32 : 64, TB = BR * L::ROWB;
   __shared__ __align__(16) char smem[2 * TB];
   __shared__ __align__(16) float st[2][BR];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-  const int kvh = blockIdx.x % a.hkv, G = a.hq / a.hkv;
-  const Tile t = find_tile(a.cu_k, a.nseq, a.total_k, 1, BK, blockIdx.x / a.hkv, false);
+  const int G = a.group.d, block = a.heads.div(blockIdx.x), kvh = a.heads.mod(blockIdx.x, block);
+  const Tile t = find_tile(a.cu_k, a.nseq, a.total_k, 1, BK, block, false);
   if (t.seq < 0) return;
   int q0, lq;
   seq_rows(a.cu_q, a.nseq, a.total_q, t.seq, q0, lq);
@@ -749,8 +766,8 @@ __global__ void __launch_bounds__(NT, 1) k_attn_packed_dkv(const hv_attn_packed_
   const int first_tok = a.causal ? max(t.tile * BK - late, 0) : 0;
   const int first_mine = a.causal ? key - late : 0;      // first token that sees this lane's key
   const int wave_last = a.causal ? t.tile * BK + wave * 32 + 31 - late : 0;   // token that sees all of the wave's keys
-  const long rows = (long)lq * G;
-  const long r0 = (long)first_tok * G / BR * BR;
+  const int rows = lq * G;
+  const int r0 = first_tok * G / BR * BR;
   const float c2 = a.scale * LOG2E;
 
   f32x16 dk[L::NDT], dv[L::NDT];
@@ -762,20 +779,21 @@ __global__ void __launch_bounds__(NT, 1) k_attn_packed_dkv(const hv_attn_packed_
   const long sbase = (long)q0 * a.hq + (long)kvh * G;
   Stage<T, DP, BR> sq, sg;
   float stat = 0.f;
-  auto fetch = [&](long rr) {
+  auto fetch = [&](int rr) {
     sq.load(a.d, [&](int row) {
-      const long x = rr + row;
-      return x < rows ? qp + (x / G) * a.q_row + (x % G) * a.q_head : nullptr;
+      const int x = rr + row, tk = a.group.div(x);
+      return x < rows ? qp + tk * a.q_row + a.group.mod(x, tk) * a.q_head : nullptr;
     });
     sg.load(a.d, [&](int row) {
-      const long x = rr + row;
-      return x < rows ? gp + (x / G) * a.do_row + (x % G) * a.do_head : nullptr;
+      const int x = rr + row, tk = a.group.div(x);
+      return x < rows ? gp + tk * a.do_row + a.group.mod(x, tk) * a.do_head : nullptr;
     });
     if (threadIdx.x < 2 * BR) {
-      const long x = rr + (threadIdx.x & (BR - 1));
+      const int x = rr + (threadIdx.x & (BR - 1));
       stat = 0.f;
       if (x < rows) {
-        const long at = sbase + (x / G) * a.hq + x % G;
+        const int tk = a.group.div(x);
+        const long at = sbase + (long)tk * a.hq + a.group.mod(x, tk);
         if (threadIdx.x < BR) {
           const float le = a.lse[at];
           stat = le == NEG_INF ? 0.f : -le * LOG2E;
@@ -786,7 +804,7 @@ __global__ void __launch_bounds__(NT, 1) k_attn_packed_dkv(const hv_attn_packed_
     }
   };
   if (r0 < rows) fetch(r0);
-  for (long rr = r0; rr < rows; rr += BR) {
+  for (int rr = r0; rr < rows; rr += BR) {
     __syncthreads();
     sq.store(smem);
     sg.store(smem + TB);
@@ -795,7 +813,7 @@ __global__ void __launch_bounds__(NT, 1) k_attn_packed_dkv(const hv_attn_packed_
     if (rr + BR < rows) fetch(rr + BR);
 #pragma unroll 1
     for (int j = 0; j < BR; j += 32) {
-      const long rj = rr + j;
+      const int rj = rr + j;
       if (rj >= rows) break;
       const char* tq = smem + j * L::ROWB;
       const char* tg = tq + TB;
@@ -805,7 +823,7 @@ __global__ void __launch_bounds__(NT, 1) k_attn_packed_dkv(const hv_attn_packed_
         s = mma16(view.rows(tq, i), kf[i], s);
         dp = mma16(view.rows(tg, i), vf[i], dp);
       }
-      const bool edge = rj + 32 > rows || (int)(rj / G) < wave_last;
+      const bool edge = rj + 32 > rows || a.group.div(rj) < wave_last;
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
         const f32x4 le = *(const f32x4*)&st[0][j + 8 * y + 4 * h];
@@ -814,8 +832,8 @@ __global__ void __launch_bounds__(NT, 1) k_attn_packed_dkv(const hv_attn_packed_
         for (int x = 0; x < 4; ++x) {
           float p = __builtin_amdgcn_exp2f(fmaf(s[4 * y + x], c2, le[x]));
           if (edge) {
-            const long at = rj + 8 * y + 4 * h + x;
-            if (at >= rows || (int)(at / G) < first_mine) p = 0.f;
+            const int at = rj + 8 * y + 4 * h + x;
+            if (at >= rows || a.group.div(at) < first_mine) p = 0.f;
           }
           s[4 * y + x] = p;
           dp[4 * y + x] = p * (dp[4 * y + x] - dl[x]);
@@ -849,7 +867,7 @@ int check_shape(const hv_attn_packed_args* a) {
   if (a->hq <= 0 || a->hkv <= 0 || a->hq % a->hkv || a->nseq < 0 || a->total_q < 0 || a->total_k < 0) return HV_EINVAL;
   if (!(a->scale > 0.f) || a->scale > 3.0e38f) return HV_EINVAL;
   if (a->d <= 0 || a->d % 8 || a->d > 128 || a->hq > 1024) return HV_EUNSUPPORTED;
-  if (a->total_q >= (1L << 30) || a->total_k >= (1L << 30)) return HV_EUNSUPPORTED;
+  if (a->total_q >= (1L << 30) || a->total_q * (a->hq / a->hkv) >= (1L << 30) || a->total_k >= (1L << 30)) return HV_EUNSUPPORTED;
   return HV_OK;
 }
 
@@ -880,7 +898,7 @@ int part_keys(const hv_attn_packed_args& a) {
 }
 size_t part_rows(const hv_attn_packed_args& a, int n) { return (size_t)((a.total_k + n - 1) / n) * a.total_q * a.hq; }
 
-template <typename T, int DP> void launch_keys(const hv_attn_packed_args& a, int n, hipStream_t s) {
+template <typename T, int DP> void launch_keys(const Args& a, int n, hipStream_t s) {
   const size_t rows = part_rows(a, n);
   float* po = (float*)a.work;
   float4* pml = (float4*)(po + rows * a.d);
@@ -889,13 +907,13 @@ template <typename T, int DP> void launch_keys(const hv_attn_packed_args& a, int
   k_attn_packed_join<T><<<hv_cdiv(a.total_q * a.hq, 4), NT, 0, s>>>(a, n, po, pml);
 }
 
-template <typename T, int DP> void launch_forward(const hv_attn_packed_args& a, unsigned blocks, hipStream_t s) {
+template <typename T, int DP> void launch_forward(const Args& a, unsigned blocks, hipStream_t s) {
   if (a.lse != nullptr || a.out_low != nullptr) k_attn_packed<T, DP, true><<<blocks, NT, 0, s>>>(a);
   else k_attn_packed<T, DP, false><<<blocks, NT, 0, s>>>(a);
 }
 
 template <typename T, int DP>
-void launch_backward(const hv_attn_packed_args& a, unsigned bq, unsigned bk, float* delta, hipStream_t s) {
+void launch_backward(const Args& a, unsigned bq, unsigned bk, float* delta, hipStream_t s) {
   if (a.total_q) {
     k_attn_packed_delta<T><<<(unsigned)min((a.total_q * a.hq + 15) / 16, 1L << 20), NT, 0, s>>>(a, delta);
     if (a.dq) k_attn_packed_dq<T, DP><<<bq, NT, 0, s>>>(a, delta);
@@ -933,9 +951,9 @@ extern "C" int hv_attn_packed(const hv_attn_packed_args* a, hv_stream_t stream) 
   if (n) {
     if (a->work == nullptr || ((uintptr_t)a->work & 15) || tile_bound(a->total_k, a->nseq, 1, n) * a->hkv >= MAX_BLOCKS)
       return HV_EINVAL;
-    HV_DISPATCH(a->dtype, HV_HEAD_DIM(a->d, launch_keys, *a, n, s));
+    HV_DISPATCH(a->dtype, HV_HEAD_DIM(a->d, launch_keys, Args(*a), n, s));
   } else
-    HV_DISPATCH(a->dtype, HV_HEAD_DIM(a->d, launch_forward, *a, (unsigned)blocks, s));
+    HV_DISPATCH(a->dtype, HV_HEAD_DIM(a->d, launch_forward, Args(*a), (unsigned)blocks, s));
   HV_CHECK_LAUNCH();
   hv_diag_count(HV_KF_ATTN_PACKED);
   return HV_OK;
@@ -958,7 +976,7 @@ extern "C" int hv_attn_packed_backward(const hv_attn_packed_args* a, hv_stream_t
   const long bk = tile_bound(a->total_k, a->nseq, 1, 128) * a->hkv;
   if (bq >= MAX_BLOCKS || bk >= MAX_BLOCKS) return HV_EUNSUPPORTED;
   hipStream_t s = (hipStream_t)stream;
-  HV_DISPATCH(a->dtype, HV_HEAD_DIM(a->d, launch_backward, *a, (unsigned)bq, (unsigned)bk, (float*)a->work, s));
+  HV_DISPATCH(a->dtype, HV_HEAD_DIM(a->d, launch_backward, Args(*a), (unsigned)bq, (unsigned)bk, (float*)a->work, s));
   HV_CHECK_LAUNCH();
   hv_diag_count(HV_KF_ATTN_PACKED);
   return HV_OK;
