@@ -217,26 +217,32 @@ __device__ __forceinline__ void seq_rows(const int* __restrict__ cu, int nseq, l
   if (len < 0) len = 0;
 }
 
-// 16-byte chunks of ROWS tile rows -> registers -> LDS; source row `row` of the tile is src(row)'s address or
-// null (zeros), chunks at columns >= d are zero
-template <typename T, int DP, int ROWS> struct Stage {
+// 16 bytes per lane from memory to LDS at lds + 16 lane, without registers in between.  Inline assembly, so that the
+// compiler does not wait for it before the next LDS read: arrived() does, once per tile.
+__device__ __forceinline__ void dma16(const void* src, unsigned lds) {
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
+#pragma clang diagnostic pop
+}
+__device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ unsigned lds_at(const void* p) {
+  return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const unsigned char*)p;
+}
+
+// ROWS tile rows into LDS, by the whole block: 64 chunks a wave instruction, permuted on the source side.  src(row) is the
+// address of a row; it has to be one that may be read also for rows behind the last (the callers clamp: what such rows
+// hold is masked).  Chunks at columns >= d are read from column 0: the other operand is 0 there.
+template <typename T, int DP, int ROWS> struct Dma {
   using L = Lay<T, DP>;
-  static constexpr int N = ROWS * L::CH / NT;
+  static constexpr int N = ROWS * L::CH / NT;            // instructions of a wave
   static_assert(N * NT == ROWS * L::CH, "whole chunks per thread");
-  u32x4 r[N];
-  template <typename F> __device__ __forceinline__ void load(int d, F src) {
+  template <typename F> static __device__ __forceinline__ void issue(unsigned lds, int d, F src) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const int i = threadIdx.x + n * NT, row = i / L::CH, c = i % L::CH;
-      const T* p = src(row);
-      r[n] = (p != nullptr && c * L::EPC < d) ? *(const u32x4*)(p + c * L::EPC) : u32x4{0, 0, 0, 0};
-    }
-  }
-  __device__ __forceinline__ void store(char* tile) const {
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const int i = threadIdx.x + n * NT, row = i / L::CH, c = i % L::CH;
-      *(u32x4*)(tile + row * L::ROWB + ((c ^ L::f(row)) << 4)) = r[n];
+      const int i = (wave * N + n) * 64 + lane, row = i / L::CH, c = (i % L::CH) ^ L::f(row);
+      dma16(src(row) + (c * L::EPC < d ? c * L::EPC : 0), lds + (wave * N + n) * 1024);
     }
   }
 };
@@ -263,6 +269,20 @@ template <typename T, int DP> __device__ __forceinline__ void load_row(Frag<T>* 
 #pragma unroll
         for (int x = 0; x < 4; ++x) f[s].v[e + x] = a[x];
       }
+    }
+  }
+}
+
+// Have the operands in registers from here on.  Without it the compiler places its wait for their loads at the first use
+// inside the tile loop, where it would also wait for the tile that is on its way.
+template <typename T, int N> __device__ __forceinline__ void settle(Frag<T> (&f)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if constexpr (sizeof(T) == 2) {
+      asm volatile("" : "+v"(f[i].v));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) asm volatile("" : "+v"(f[i].v[e]));
     }
   }
 }
@@ -299,8 +319,8 @@ __device__ __forceinline__ f32x16 zero16() {
 template <typename T, int DP, bool TRAIN>
 __global__ void __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) k_attn_packed(const Args a) {
   using L = Lay<T, DP>;
-  constexpr int BM = 128, BN = 64, TB = BN * L::ROWB;
-  __shared__ __align__(16) char smem[2 * TB];
+  constexpr int BM = 128, BN = L::ROWB > 256 ? 32 : 64, TB = BN * L::ROWB, NJ = BN / 32;
+  __shared__ __align__(16) char smem[4 * TB];          // K and V, two buffers
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
   const int G = a.group.d, block = a.heads.div(blockIdx.x), kvh = a.heads.mod(blockIdx.x, block);
   const Tile t = find_tile(a.cu_q, a.nseq, a.total_q, G, BM, block, a.causal != 0);
@@ -329,6 +349,7 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) k_att
   const int qh = kvh * G + g;
   Frag<T> q[L::NS];
   load_row<T, DP>(q, real ? (const T*)a.q + qrow * a.q_row + (long)qh * a.q_head : nullptr, a.d, h);
+  settle(q);
   const T* kp = (const T*)a.k + (long)k0 * a.k_row + (long)kvh * a.k_head;
   const T* vp = (const T*)a.v + (long)k0 * a.v_row + (long)kvh * a.v_head;
 
@@ -340,28 +361,31 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) k_att
   const View<T, DP> view(lane);
   const int ntile = (lim_blk + BN) / BN;
 
-  Stage<T, DP, BN> sk, sv;
+  const unsigned lds0 = lds_at(smem);
   auto fetch = [&](int kt) {
-    sk.load(a.d, [&](int row) { const int j = kt * BN + row; return j <= lim_blk ? kp + (long)j * a.k_row : nullptr; });
-    sv.load(a.d, [&](int row) { const int j = kt * BN + row; return j <= lim_blk ? vp + (long)j * a.v_row : nullptr; });
+    const unsigned at = lds0 + (kt & 1) * 2 * TB;
+    Dma<T, DP, BN>::issue(at, a.d, [&](int row) { return kp + (long)min(kt * BN + row, lim_blk) * a.k_row; });
+    Dma<T, DP, BN>::issue(at + TB, a.d, [&](int row) { return vp + (long)min(kt * BN + row, lim_blk) * a.v_row; });
   };
   if (ntile > 0) fetch(0);
   for (int kt = 0; kt < ntile; ++kt) {
-    __syncthreads();
-    sk.store(smem);
-    sv.store(smem + TB);
-    __syncthreads();
+    arrived();
+    __syncthreads();                                     // tile kt is here, the other buffer is no longer read
+    const char* tk = smem + (kt & 1) * 2 * TB;
+    const char* tv = tk + TB;
     if (kt + 1 < ntile) fetch(kt + 1);
     if (kt * BN > lim_hi) continue;
-    f32x16 s[2] = {zero16(), zero16()};
+    f32x16 s[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) s[j] = zero16();
 #pragma unroll
     for (int i = 0; i < L::NS; ++i) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) s[j] = mma16(view.rows(smem + j * 32 * L::ROWB, i), q[i], s[j]);
+      for (int j = 0; j < NJ; ++j) s[j] = mma16(view.rows(tk + j * 32 * L::ROWB, i), q[i], s[j]);
     }
     if (kt * BN + BN - 1 > lim_lo) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < NJ; ++j)
 #pragma unroll
         for (int x = 0; x < 16; ++x)
           if (kt * BN + 32 * j + 8 * (x >> 2) + 4 * h + (x & 3) > lim) s[j][x] = NEG_INF;
@@ -370,7 +394,9 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) k_att
 #pragma unroll
     for (int x = 1; x < 16; ++x) top = fmaxf(top, s[0][x]);
 #pragma unroll
-    for (int x = 0; x < 16; ++x) top = fmaxf(top, s[1][x]);
+    for (int j = 1; j < NJ; ++j)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) top = fmaxf(top, s[j][x]);
     top = fmaxf(top, other_half(top));
     // the running maximum moves only when a score passes it by 8 powers of two: weights stay below 2^8 and
     // the accumulators are seldom rescaled
@@ -387,24 +413,24 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) k_att
     }
     const float mc = m == NEG_INF ? 0.f : -m * c2;
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < NJ; ++j)
 #pragma unroll
       for (int x = 0; x < 16; ++x) s[j][x] = __builtin_amdgcn_exp2f(fmaf(s[j][x], c2, mc));
     if constexpr (TRAIN && sizeof(T) == 2) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < NJ; ++j)
 #pragma unroll
         for (int x = 0; x < 16; ++x) lt += s[j][x];
     }
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < NJ; ++j)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const Frag<T> p = from_acc<T>(s[j], i);
         l = add_sum(p, l);
 #pragma unroll
         for (int dt = 0; dt < L::NDT; ++dt)
-          o[dt] = mma16(view.cols(smem + TB + (32 * j + 16 * i) * L::ROWB, dt), p, o[dt]);
+          o[dt] = mma16(view.cols(tv + (32 * j + 16 * i) * L::ROWB, dt), p, o[dt]);
       }
   }
   if (!real) return;
@@ -661,8 +687,8 @@ __global__ void __launch_bounds__(NT) k_attn_packed_delta(const Args a, float* _
 template <typename T, int DP>
 __global__ void __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) k_attn_packed_dq(const Args a, const float* __restrict__ delta) {
   using L = Lay<T, DP>;
-  constexpr int BM = 128, BN = 64, TB = BN * L::ROWB;
-  __shared__ __align__(16) char smem[2 * TB];
+  constexpr int BM = 128, BN = L::ROWB > 256 ? 32 : 64, TB = BN * L::ROWB;
+  __shared__ __align__(16) char smem[4 * TB];          // K and V, two buffers
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
   const int G = a.group.d, block = a.heads.div(blockIdx.x), kvh = a.heads.mod(blockIdx.x, block);
   const Tile t = find_tile(a.cu_q, a.nseq, a.total_q, G, BM, block, a.causal != 0);
@@ -689,10 +715,13 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) k_att
   Frag<T> q[L::NS], go[L::NS];
   load_row<T, DP>(q, real ? (const T*)a.q + qrow * a.q_row + (long)qh * a.q_head : nullptr, a.d, h);
   load_row<T, DP>(go, real ? (const T*)a.dout + qrow * a.do_row + (long)qh * a.do_head : nullptr, a.d, h);
+  settle(q);
+  settle(go);
   const float c2 = a.scale * LOG2E;
   float le = real ? a.lse[qrow * a.hq + qh] : 0.f;
   le = le == NEG_INF ? 0.f : -le * LOG2E;
-  const float dl = real ? delta[qrow * a.hq + qh] : 0.f;
+  float dl = real ? delta[qrow * a.hq + qh] : 0.f;
+  asm volatile("" : "+v"(le), "+v"(dl));
   const T* kp = (const T*)a.k + (long)k0 * a.k_row + (long)kvh * a.k_head;
   const T* vp = (const T*)a.v + (long)k0 * a.v_row + (long)kvh * a.v_head;
 
@@ -701,27 +730,28 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) k_att
   for (int i = 0; i < L::NDT; ++i) dq[i] = zero16();
   const View<T, DP> view(lane);
   const int ntile = (lim_blk + BN) / BN;
-  Stage<T, DP, BN> sk, sv;
+  const unsigned lds0 = lds_at(smem);
   auto fetch = [&](int kt) {
-    sk.load(a.d, [&](int row) { const int j = kt * BN + row; return j <= lim_blk ? kp + (long)j * a.k_row : nullptr; });
-    sv.load(a.d, [&](int row) { const int j = kt * BN + row; return j <= lim_blk ? vp + (long)j * a.v_row : nullptr; });
+    const unsigned at = lds0 + (kt & 1) * 2 * TB;
+    Dma<T, DP, BN>::issue(at, a.d, [&](int row) { return kp + (long)min(kt * BN + row, lim_blk) * a.k_row; });
+    Dma<T, DP, BN>::issue(at + TB, a.d, [&](int row) { return vp + (long)min(kt * BN + row, lim_blk) * a.v_row; });
   };
   if (ntile > 0) fetch(0);
   for (int kt = 0; kt < ntile; ++kt) {
-    __syncthreads();
-    sk.store(smem);
-    sv.store(smem + TB);
-    __syncthreads();
+    arrived();
+    __syncthreads();                                     // tile kt is here, the other buffer is no longer read
+    const char* tk = smem + (kt & 1) * 2 * TB;
+    const char* tv = tk + TB;
     if (kt + 1 < ntile) fetch(kt + 1);
 #pragma unroll 1
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < BN / 32; ++j) {
       const int key = kt * BN + 32 * j;
       if (key > lim_hi) break;
       f32x16 s = zero16(), dp = zero16();
 #pragma unroll
       for (int i = 0; i < L::NS; ++i) {
-        s = mma16(view.rows(smem + j * 32 * L::ROWB, i), q[i], s);
-        dp = mma16(view.rows(smem + TB + j * 32 * L::ROWB, i), go[i], dp);
+        s = mma16(view.rows(tk + j * 32 * L::ROWB, i), q[i], s);
+        dp = mma16(view.rows(tv + j * 32 * L::ROWB, i), go[i], dp);
       }
       if (key + 31 > lim_lo) {
 #pragma unroll
@@ -735,7 +765,7 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) k_att
         const Frag<T> p = from_acc<T>(s, i);
 #pragma unroll
         for (int dt = 0; dt < L::NDT; ++dt)
-          dq[dt] = mma16(view.cols(smem + (32 * j + 16 * i) * L::ROWB, dt), p, dq[dt]);
+          dq[dt] = mma16(view.cols(tk + (32 * j + 16 * i) * L::ROWB, dt), p, dq[dt]);
       }
     }
   }
@@ -744,11 +774,11 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) k_att
 
 // dK, dV: a wave holds 32 keys and walks over the packed rows of its sequence (all heads of the group)
 template <typename T, int DP>
-__global__ void __launch_bounds__(NT, DP == 128 || sizeof(T) == 4 ? 1 : 2) k_attn_packed_dkv(const Args a, const float* __restrict__ delta) {
+__global__ void __launch_bounds__(NT, DP * sizeof(T) >= 256 ? 1 : 2) k_attn_packed_dkv(const Args a, const float* __restrict__ delta) {
   using L = Lay<T, DP>;
-  constexpr int BK = 128, BR = L::ROWB >= 512 ? 32 : 64, TB = BR * L::ROWB;
-  __shared__ __align__(16) char smem[2 * TB];
-  __shared__ __align__(16) float st[2][BR];
+  constexpr int BK = 128, BR = L::ROWB > 256 ? 32 : 64, TB = BR * L::ROWB;
+  __shared__ __align__(16) char smem[4 * TB];          // Q and dO, two buffers
+  __shared__ __align__(16) float st[2][2][BR];         // -lse log2 e and delta of the rows
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
   const int G = a.group.d, block = a.heads.div(blockIdx.x), kvh = a.heads.mod(blockIdx.x, block);
   const Tile t = find_tile(a.cu_k, a.nseq, a.total_k, 1, BK, block, false);
@@ -761,6 +791,8 @@ __global__ void __launch_bounds__(NT, DP == 128 || sizeof(T) == 4 ? 1 : 2) k_att
   Frag<T> kf[L::NS], vf[L::NS];
   load_row<T, DP>(kf, real ? (const T*)a.k + krow * a.k_row + (long)kvh * a.k_head : nullptr, a.d, h);
   load_row<T, DP>(vf, real ? (const T*)a.v + krow * a.v_row + (long)kvh * a.v_head : nullptr, a.d, h);
+  settle(kf);
+  settle(vf);
   const int late = t.len - lq;
   // causal: row (token i) sees key j iff i >= j - late
   const int first_tok = a.causal ? max(t.tile * BK - late, 0) : 0;
@@ -777,16 +809,16 @@ __global__ void __launch_bounds__(NT, DP == 128 || sizeof(T) == 4 ? 1 : 2) k_att
   const T* qp = (const T*)a.q + (long)q0 * a.q_row + (long)kvh * G * a.q_head;
   const T* gp = (const T*)a.dout + (long)q0 * a.do_row + (long)kvh * G * a.do_head;
   const long sbase = (long)q0 * a.hq + (long)kvh * G;
-  Stage<T, DP, BR> sq, sg;
+  const unsigned lds0 = lds_at(smem);
   float stat = 0.f;
-  auto fetch = [&](int rr) {
-    sq.load(a.d, [&](int row) {
-      const int x = rr + row, tk = a.group.div(x);
-      return x < rows ? qp + tk * a.q_row + a.group.mod(x, tk) * a.q_head : nullptr;
+  auto fetch = [&](int rr, int buf) {
+    Dma<T, DP, BR>::issue(lds0 + buf * 2 * TB, a.d, [&](int row) {
+      const int x = min(rr + row, rows - 1), tk = a.group.div(x);
+      return qp + tk * a.q_row + a.group.mod(x, tk) * a.q_head;
     });
-    sg.load(a.d, [&](int row) {
-      const int x = rr + row, tk = a.group.div(x);
-      return x < rows ? gp + tk * a.do_row + a.group.mod(x, tk) * a.do_head : nullptr;
+    Dma<T, DP, BR>::issue(lds0 + buf * 2 * TB + TB, a.d, [&](int row) {
+      const int x = min(rr + row, rows - 1), tk = a.group.div(x);
+      return gp + tk * a.do_row + a.group.mod(x, tk) * a.do_head;
     });
     if (threadIdx.x < 2 * BR) {
       const int x = rr + (threadIdx.x & (BR - 1));
@@ -803,19 +835,17 @@ __global__ void __launch_bounds__(NT, DP == 128 || sizeof(T) == 4 ? 1 : 2) k_att
       }
     }
   };
-  if (r0 < rows) fetch(r0);
-  for (int rr = r0; rr < rows; rr += BR) {
+  if (r0 < rows) fetch(r0, 0);
+  for (int rr = r0, buf = 0; rr < rows; rr += BR, buf ^= 1) {
+    if (threadIdx.x < 2 * BR) st[buf][threadIdx.x / BR][threadIdx.x & (BR - 1)] = stat;
+    arrived();
     __syncthreads();
-    sq.store(smem);
-    sg.store(smem + TB);
-    if (threadIdx.x < 2 * BR) st[threadIdx.x / BR][threadIdx.x & (BR - 1)] = stat;
-    __syncthreads();
-    if (rr + BR < rows) fetch(rr + BR);
+    if (rr + BR < rows) fetch(rr + BR, buf ^ 1);
 #pragma unroll 1
     for (int j = 0; j < BR; j += 32) {
       const int rj = rr + j;
       if (rj >= rows) break;
-      const char* tq = smem + j * L::ROWB;
+      const char* tq = smem + buf * 2 * TB + j * L::ROWB;
       const char* tg = tq + TB;
       f32x16 s = zero16(), dp = zero16();
 #pragma unroll
@@ -826,18 +856,22 @@ __global__ void __launch_bounds__(NT, DP == 128 || sizeof(T) == 4 ? 1 : 2) k_att
       const bool edge = rj + 32 > rows || a.group.div(rj) < wave_last;
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
-        const f32x4 le = *(const f32x4*)&st[0][j + 8 * y + 4 * h];
-        const f32x4 dl = *(const f32x4*)&st[1][j + 8 * y + 4 * h];
+        const f32x4 le = *(const f32x4*)&st[buf][0][j + 8 * y + 4 * h];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          float p = __builtin_amdgcn_exp2f(fmaf(s[4 * y + x], c2, le[x]));
-          if (edge) {
-            const int at = rj + 8 * y + 4 * h + x;
-            if (at >= rows || a.group.div(at) < first_mine) p = 0.f;
-          }
-          s[4 * y + x] = p;
-          dp[4 * y + x] = p * (dp[4 * y + x] - dl[x]);
+        for (int x = 0; x < 4; ++x) s[4 * y + x] = __builtin_amdgcn_exp2f(fmaf(s[4 * y + x], c2, le[x]));
+      }
+      if (edge) {
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          const int at = rj + 8 * (x >> 2) + 4 * h + (x & 3);
+          s[x] = at >= rows || a.group.div(at) < first_mine ? 0.f : s[x];
         }
+      }
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const f32x4 dl = *(const f32x4*)&st[buf][1][j + 8 * y + 4 * h];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) dp[4 * y + x] = s[4 * y + x] * (dp[4 * y + x] - dl[x]);
       }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
