@@ -14,8 +14,8 @@
 // The backward uses the same two moves for dQ^T += K^T dS^T, dV^T += dO^T P and dK^T += Q^T dS.
 //
 // LDS tiles are rows of DP elements (DP = d rounded up to 32 / 64 / 128, columns >= d zero) whose 16-byte
-// chunks are permuted by a function of the row, so that both the row reads (8 rows of one chunk) and the
-// transposing reads (4 rows of two chunks) touch every bank once.
+// chunks are permuted by a function of the row (Lay::f), so that the row reads (16 rows of one chunk) and the
+// transposing reads (4 rows of four chunks) spread over the banks.
 #include "hv_common.h"
 
 namespace {
@@ -64,8 +64,13 @@ template <typename T, int DP> struct Lay {               // an LDS tile
   static constexpr int CH = ROWB / 16;                   // its 16-byte chunks
   static constexpr int EPC = 16 / (int)sizeof(T);        // elements of a chunk
   static constexpr int NS = DP / 16, NDT = DP / 32;      // 16-column steps, 32-column tiles
-  static __device__ __forceinline__ int f(int row) {     // chunk permutation of a row (rows = 0 mod 8: 0)
-    return CH >= 8 ? ((row & 3) << 1) | ((row >> 2) & 1) : (row & 2) | ((row >> 2) & 1);
+  // chunk permutation of a row (a row of 0 mod 16: none).  CH >= 16: 16 rows' equal chunks, and 4 rows' aligned groups of
+  // 4, lie in 256 different bytes, the width of an LDS access (permuted over 128 bytes only: half the LDS rate, 127 against
+  // 228 bytes a clock and CU; the forward gains 2 %).  Shorter rows: over 128 bytes, so that a row and the row 8 below it
+  // are permuted alike and share an address (64 columns: 92 us, over 256 bytes 98 us, causal ragged batch of 8569 rows).
+  static constexpr __device__ __forceinline__ int f(int row) {
+    return CH >= 16 ? ((row & 3) << 2) | ((row >> 2) & 3)
+                    : CH == 8 ? ((row & 3) << 1) | ((row >> 2) & 1) : (row & 2) | ((row >> 2) & 1);
   }
 };
 
@@ -84,7 +89,7 @@ template <typename T, int DP> struct View {
     } else {
       row_x = ((2 * h) ^ L::f(m)) << 4;
       tr_base = 4 * h * L::ROWB + (m & 3) * 4;
-      tr_x = ((m >> 2) ^ h) << 4;                        // f(4 h + e) = 2 e | h; the 2 e part is added per element
+      tr_x = ((m >> 2) ^ h) << 4;                        // f(4 h) = h here, the rest of the row per element
     }
   }
   // operand over columns 16 s .. 16 s + 15 of the 32 rows from `tile` (a multiple of 32 rows into the tile)
@@ -100,22 +105,23 @@ template <typename T, int DP> struct View {
     }
     return r;
   }
-  // transposed operand: columns 32 dt .. 32 dt + 31 as rows, the 16 tile rows from `tile` (a multiple of 8 rows
+  // transposed operand: columns 32 dt .. 32 dt + 31 as rows, the 16 tile rows from `tile` (a multiple of 16 rows
   // into the tile) as contraction slots
   __device__ __forceinline__ Frag<T> cols(const char* tile, int dt) const {
     Frag<T> r;
     if constexpr (sizeof(T) == 2) {
       typedef __attribute__((address_space(3))) s16x4 lds4;
-      const char* p = tile + tr_base + (tr_x ^ (dt << 6));
+      const char* p = tile + tr_base;
+      const int x = tr_x ^ (dt << 6);
       union { s16x4 q[2]; bf16x8 v; } u;
-      u.q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p));
-      u.q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 8 * L::ROWB));
+      u.q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + x));
+      u.q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 8 * L::ROWB + (x ^ (L::f(8) << 4))));
       r.v = u.v;
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         r.v[e] = *(const float*)(tile + (8 * (e >> 2) + (e & 3)) * L::ROWB + tr_base +
-                                 (tr_x ^ (dt << 7) ^ ((e & 3) << 5)));
+                                 (tr_x ^ (dt << 7) ^ (L::f(8 * (e >> 2) + (e & 3)) << 4)));
     }
     return r;
   }
@@ -139,9 +145,9 @@ template <typename T> __device__ __forceinline__ Frag<T> from_acc(const f32x16& 
 // sum of the 8 values as the product sees them (rounded to T), added to c
 __device__ __forceinline__ float add_sum(const Frag<unsigned short>& p, float c) {
   const u32x4 u = __builtin_bit_cast(u32x4, p.v);
+  const bf16x2 one = {(__bf16)1.f, (__bf16)1.f};
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    c += __uint_as_float(u[e] << 16) + __uint_as_float(u[e] & 0xffff0000u);
+  for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, (uint32_t)u[e]), one, c, false);
   return c;
 }
 __device__ __forceinline__ float add_sum(const Frag<float>& p, float c) {
