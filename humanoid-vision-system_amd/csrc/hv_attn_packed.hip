@@ -232,6 +232,13 @@ __device__ __forceinline__ void dma16(const void* src, unsigned lds) {
   asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
 #pragma clang diagnostic pop
 }
+// the same from base + off, base the same for the whole wave
+__device__ __forceinline__ void dma16_at(const void* base, unsigned off, unsigned lds) {
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
+#pragma clang diagnostic pop
+}
 __device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ unsigned lds_at(const void* p) {
   return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const unsigned char*)p;
@@ -283,38 +290,31 @@ template <typename T, int DP, int BN> struct KeyTiles : Dma<T, DP, BN> {
   }
 };
 
-// Q or dO tiles of BR packed rows (token r / G, head r % G), from the tile of the last rows backwards
+// Q or dO tiles of `used` packed rows, the largest multiple of the group G in BR (so that a tile holds whole tokens), from
+// the one with the last rows backwards.  A lane's chunks lie at the same 32-bit offsets from the tile's first token in every
+// tile, so a tile's address is one scalar addition; only the last tile's rows have to be held below `rows`.
 template <typename T, int DP, int BR> struct RowTiles : Dma<T, DP, BR> {
   using B = Dma<T, DP, BR>;
   const T* base;
-  long row_stride, head_stride, step, wrap;
-  int g[B::N], G, left;
-  __device__ __forceinline__ RowTiles(const T* p, long row, long head, const FastDiv& group)
-      : base(p), row_stride(row), head_stride(head), G(group.d), left(BR - group.div(BR) * (int)group.d) {
-    step = group.div(BR) * row + left * head;
-    wrap = row - G * head;
-  }
-  // the tile that starts at row r (a multiple of BR) and holds the last of `rows` rows; then next() is the one before
-  __device__ __forceinline__ void last(int r, int rows, int d, const FastDiv& group, unsigned lds) {
+  unsigned off[B::N];
+  __device__ __forceinline__ RowTiles(const T* p, long row, long head, int used, int d, const FastDiv& group) : base(p) {
 #pragma unroll
     for (int n = 0; n < B::N; ++n) {
-      const int x = r + B::row(n), y = min(x, rows - 1), tx = group.div(x), ty = group.div(y);
-      B::send(base + ty * row_stride + group.mod(y, ty) * head_stride + B::col(n, d), lds, n);
-      g[n] = group.mod(x, tx);
-      B::at[n] = base + tx * row_stride + g[n] * head_stride + B::col(n, d);
-      back(n);
+      const int x = min(B::row(n), used - 1), t = group.div(x);
+      off[n] = (unsigned)((t * row + group.mod(x, t) * head + B::col(n, d)) * sizeof(T));
     }
   }
-  __device__ __forceinline__ void back(int n) {
-    g[n] -= left;
-    const bool w = g[n] < 0;
-    g[n] += w ? G : 0;
-    B::at[n] -= step + (w ? wrap : 0);
-  }
-  __device__ __forceinline__ void next(unsigned lds) {
-    B::issue(lds);
+  __device__ __forceinline__ void last(long row, long head, int r, int rows, int d, const FastDiv& group, unsigned lds) const {
 #pragma unroll
-    for (int n = 0; n < B::N; ++n) back(n);
+    for (int n = 0; n < B::N; ++n) {
+      const int x = min(r + B::row(n), rows - 1), t = group.div(x);
+      B::send(base + t * row + group.mod(x, t) * head + B::col(n, d), lds, n);
+    }
+  }
+  __device__ __forceinline__ void send_tile(long token_offset, unsigned lds) const {
+    const T* p = base + token_offset;
+#pragma unroll
+    for (int n = 0; n < B::N; ++n) dma16_at(p, off[n], lds + (B::wave() * B::N + n) * 1024);
   }
 };
 
@@ -848,10 +848,13 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) k_att
 // dK, dV: a block holds 64 keys and walks over the packed rows of its sequence (all heads of the group), 64 rows a tile:
 // waves 0 and 2 own the first 32 keys, 1 and 3 the others; 0 and 1 take a tile's first 32 rows, 2 and 3 the others, and
 // the two halves are added through LDS at the end.  (A block of 128 keys whose waves all walk over every row has the same
-// LDS traffic and half as many, twice as long blocks: 4096 + 2991 causal tokens, 4 heads, 760 us against the time below.)
+// LDS traffic and half as many, twice as long blocks: 4096 + 2991 causal tokens, 4 heads, 760 against 700 us.)  Where the
+// keys give few blocks, gridDim.y blocks share a key tile's rows and write fp32 parts that k_attn_packed_sum adds in order.
 template <typename T, int DP>
-__global__ void __launch_bounds__(NT, DP * sizeof(T) >= 256 ? 1 : 2) k_attn_packed_dkv(const Args a, const float* __restrict__ delta) {
+__global__ void __launch_bounds__(NT, DP * sizeof(T) >= 256 ? 1 : 2) k_attn_packed_dkv(const Args a, const float* __restrict__ delta,
+                                                                                          float* __restrict__ part_dk) {
   using L = Lay<T, DP>;
+  auto fence = [] { if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0); };
   constexpr int BK = KEYS, BR = 64, TB = BR * L::ROWB;
   __shared__ __align__(16) char smem[4 * TB];          // Q and dO, two buffers
   __shared__ __align__(16) float st[2][2][BR];         // -lse log2 e and delta of the rows
@@ -876,7 +879,6 @@ __global__ void __launch_bounds__(NT, DP * sizeof(T) >= 256 ? 1 : 2) k_attn_pack
   const int first_mine = a.causal ? key - late : 0;      // first token that sees this lane's key
   const int wave_last = a.causal ? t.tile * BK + kh * 32 + 31 - late : 0;   // token that sees all of the wave's keys
   const int rows = lq * G;
-  const int r0 = first_tok * G / BR * BR;
   const float c2 = a.scale * LOG2E;
 
   f32x16 dk[L::NDT], dv[L::NDT];
@@ -888,12 +890,14 @@ __global__ void __launch_bounds__(NT, DP * sizeof(T) >= 256 ? 1 : 2) k_attn_pack
   const long sbase = (long)q0 * a.hq + (long)kvh * G;
   const unsigned lds0 = lds_at(smem);
   float stat = 0.f;
-  RowTiles<T, DP, BR> sq(qp, a.q_row, a.q_head, a.group), sg(gp, a.do_row, a.do_head, a.group);
+  const int used = a.group.div(BR) * G, toks = a.group.div(BR);          // rows and tokens of a tile
+  const RowTiles<T, DP, BR> sq(qp, a.q_row, a.q_head, used, a.d, a.group), sg(gp, a.do_row, a.do_head, used, a.d, a.group);
+  const int t0 = first_tok / toks, tn = (lq + toks - 1) / toks;          // the tiles that this block needs
   auto stats = [&](int rr) {
     if (threadIdx.x < 2 * BR) {
-      const int x = rr + (threadIdx.x & (BR - 1));
+      const int slot = threadIdx.x & (BR - 1), x = rr + slot;
       stat = 0.f;
-      if (x < rows) {
+      if (x < rows && slot < used) {
         const int tk = a.group.div(x);
         const long at = sbase + (long)tk * a.hq + a.group.mod(x, tk);
         stat = threadIdx.x < BR ? a.lse[at] : delta[at];
@@ -901,62 +905,75 @@ __global__ void __launch_bounds__(NT, DP * sizeof(T) >= 256 ? 1 : 2) k_attn_pack
     }
   };
   // from the last rows, which every block of the sequence needs, backwards: blocks that run together read the same tiles
-  const int rl = (rows - 1) / BR * BR;
-  if (r0 < rows) {
-    sq.last(rl, rows, a.d, a.group, lds0);
-    sg.last(rl, rows, a.d, a.group, lds0 + TB);
-    stats(rl);
+  int tile = tn - 1 - (int)blockIdx.y;
+  const int parts = gridDim.y;
+  if (tile >= t0) {
+    sq.last(a.q_row, a.q_head, tile * used, rows, a.d, a.group, lds0);
+    sg.last(a.do_row, a.do_head, tile * used, rows, a.d, a.group, lds0 + TB);
+    stats(tile * used);
   }
-  for (int rr = rl, buf = 0; rr >= r0; rr -= BR, buf ^= 1) {
+  for (int buf = 0; tile >= t0; tile -= parts, buf ^= 1) {
+    const int rr = tile * used;
     arrived();
     if (threadIdx.x < BR) st[buf][0][threadIdx.x] = stat == NEG_INF ? 0.f : -stat * LOG2E;
     else if (threadIdx.x < 2 * BR) st[buf][1][threadIdx.x - BR] = stat;
     __syncthreads();
-    if (rr > r0) {
+    if (tile - parts >= t0) {
       const unsigned at = lds0 + (buf ^ 1) * 2 * TB;
-      sq.next(at);
-      sg.next(at + TB);
-      stats(rr - BR);
+      sq.send_tile((long)(tile - parts) * toks * a.q_row, at);
+      sg.send_tile((long)(tile - parts) * toks * a.do_row, at + TB);
+      stats((tile - parts) * used);
     }
     const int j = rh * 32, rj = rr + j;
-    if (rj < rows) {
-      const char* tq = smem + buf * 2 * TB + j * L::ROWB;
-      const char* tg = tq + TB;
-      f32x16 s = zero16(), dp = zero16();
+    const char* tq = smem + buf * 2 * TB + j * L::ROWB;
+    const char* tg = tq + TB;
+    // All operands of a product are on their way before its first instruction, the second products' during the first ones:
+    // one wave per SIMD has nobody else to fill the LDS latency (each read just before its use: 472 us against the below).
+    f32x16 s = zero16(), dp = zero16();
+    {
+      Frag<T> x[L::NS], y[L::NS];
 #pragma unroll
-      for (int i = 0; i < L::NS; ++i) {
-        s = mma16(view.rows(tq, i), kf[i], s);
-        dp = mma16(view.rows(tg, i), vf[i], dp);
+      for (int i = 0; i < L::NS; ++i) { x[i] = view.rows(tq, i); y[i] = view.rows(tg, i); }
+      fence();
+#pragma unroll
+      for (int i = 0; i < L::NS; ++i) { s = mma16(x[i], kf[i], s); dp = mma16(y[i], vf[i], dp); }
+    }
+    Frag<T> x[L::NDT], y[L::NDT];
+#pragma unroll
+    for (int dt = 0; dt < L::NDT; ++dt) { x[dt] = view.cols(tg, dt); y[dt] = view.cols(tq, dt); }
+    fence();
+    const int end = min(rr + used, rows);
+    const bool edge = rj + 32 > end || a.group.div(rj) < wave_last;
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const f32x4 le = *(const f32x4*)&st[buf][0][j + 8 * y + 4 * h];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) s[4 * y + x] = __builtin_amdgcn_exp2f(fmaf(s[4 * y + x], c2, le[x]));
+    }
+    if (edge) {
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        const int at = rj + 8 * (x >> 2) + 4 * h + (x & 3);
+        s[x] = at >= end || a.group.div(at) < first_mine ? 0.f : s[x];
       }
-      const bool edge = rj + 32 > rows || a.group.div(rj) < wave_last;
+    }
 #pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        const f32x4 le = *(const f32x4*)&st[buf][0][j + 8 * y + 4 * h];
+    for (int y = 0; y < 4; ++y) {
+      const f32x4 dl = *(const f32x4*)&st[buf][1][j + 8 * y + 4 * h];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) s[4 * y + x] = __builtin_amdgcn_exp2f(fmaf(s[4 * y + x], c2, le[x]));
-      }
-      if (edge) {
+      for (int x = 0; x < 4; ++x) dp[4 * y + x] = s[4 * y + x] * (dp[4 * y + x] - dl[x]);
+    }
+    {
+      Frag<T> x1[L::NDT], y1[L::NDT];
+      const Frag<T> p = from_acc<T>(s, 0), ds = from_acc<T>(dp, 0);
 #pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          const int at = rj + 8 * (x >> 2) + 4 * h + (x & 3);
-          s[x] = at >= rows || a.group.div(at) < first_mine ? 0.f : s[x];
-        }
-      }
+      for (int dt = 0; dt < L::NDT; ++dt) { x1[dt] = view.cols(tg + 16 * L::ROWB, dt); y1[dt] = view.cols(tq + 16 * L::ROWB, dt); }
+      fence();
 #pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        const f32x4 dl = *(const f32x4*)&st[buf][1][j + 8 * y + 4 * h];
+      for (int dt = 0; dt < L::NDT; ++dt) { dv[dt] = mma16(x[dt], p, dv[dt]); dk[dt] = mma16(y[dt], ds, dk[dt]); }
+      const Frag<T> p1 = from_acc<T>(s, 1), ds1 = from_acc<T>(dp, 1);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) dp[4 * y + x] = s[4 * y + x] * (dp[4 * y + x] - dl[x]);
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const Frag<T> p = from_acc<T>(s, i), ds = from_acc<T>(dp, i);
-#pragma unroll
-        for (int dt = 0; dt < L::NDT; ++dt) {
-          dv[dt] = mma16(view.cols(tg + 16 * i * L::ROWB, dt), p, dv[dt]);
-          dk[dt] = mma16(view.cols(tq + 16 * i * L::ROWB, dt), ds, dk[dt]);
-        }
-      }
+      for (int dt = 0; dt < L::NDT; ++dt) { dv[dt] = mma16(x1[dt], p1, dv[dt]); dk[dt] = mma16(y1[dt], ds1, dk[dt]); }
     }
   }
   // the second half's sums, then the first half adds them
@@ -980,10 +997,33 @@ __global__ void __launch_bounds__(NT, DP * sizeof(T) >= 256 ? 1 : 2) k_attn_pack
       dk[i][x] += half[(i * 16 + x) * 64];
       dv[i][x] += half[((L::NDT + i) * 16 + x) * 64];
     }
-  if (real) {
-    const long at = (krow * a.hkv + kvh) * a.d;
+  if (!real) return;
+  const long at = (krow * a.heads.d + kvh) * a.d;
+  if (part_dk == nullptr) {
     store_row<T, DP>((T*)a.dv + at, a.d, h, dv, 1.f);
     store_row<T, DP>((T*)a.dk + at, a.d, h, dk, a.scale);
+  } else {
+    const long all = a.total_k * a.heads.d * a.d;
+    store_row<float, DP>(part_dk + (2 * blockIdx.y) * all + at, a.d, h, dk, a.scale);
+    store_row<float, DP>(part_dk + (2 * blockIdx.y + 1) * all + at, a.d, h, dv, 1.f);
+  }
+}
+
+// dk and dv from `parts` partial sums, in their order: 8 values a thread
+template <typename T>
+__global__ void __launch_bounds__(NT) k_attn_packed_sum(const Args a, int parts, const float* __restrict__ part) {
+  const long all = a.total_k * a.heads.d * a.d;
+  for (long i = ((long)blockIdx.x * NT + threadIdx.x) * 8; i < 2 * all; i += (long)gridDim.x * NT * 8) {
+    Frag<float> s, x;
+    load8(s, part + i);
+    for (int z = 1; z < parts; ++z) {
+      load8(x, part + 2 * z * all + i);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s.v[e] += x.v[e];
+    }
+    T* to = i < all ? (T*)a.dk + i : (T*)a.dv + (i - all);
+    store4(to, s.v[0], s.v[1], s.v[2], s.v[3]);
+    store4(to + 4, s.v[4], s.v[5], s.v[6], s.v[7]);
   }
 }
 
@@ -996,7 +1036,7 @@ int check_shape(const hv_attn_packed_args* a) {
   if (a == nullptr || (a->dtype != HV_F32 && a->dtype != HV_BF16)) return HV_EINVAL;
   if (a->hq <= 0 || a->hkv <= 0 || a->hq % a->hkv || a->nseq < 0 || a->total_q < 0 || a->total_k < 0) return HV_EINVAL;
   if (!(a->scale > 0.f) || a->scale > 3.0e38f) return HV_EINVAL;
-  if (a->d <= 0 || a->d % 8 || a->d > 128 || a->hq > 1024) return HV_EUNSUPPORTED;
+  if (a->d <= 0 || a->d % 8 || a->d > 128 || a->hq > 1024 || a->hq / a->hkv > 64) return HV_EUNSUPPORTED;
   if (a->total_q >= (1L << 30) || a->total_q * (a->hq / a->hkv) >= (1L << 30) || a->total_k >= (1L << 30)) return HV_EUNSUPPORTED;
   return HV_OK;
 }
@@ -1042,13 +1082,29 @@ template <typename T, int DP> void launch_forward(const Args& a, unsigned blocks
   else k_attn_packed<T, DP, false><<<blocks, NT, 0, s>>>(a);
 }
 
+// Blocks that share the rows of a key tile (see k_attn_packed_dkv): up to four blocks per CU, eight row tiles each at least
+int row_parts(const hv_attn_packed_args& a) {
+  const int used = 64 / (a.hq / a.hkv) * (a.hq / a.hkv);
+  const long blocks = (a.total_k + KEYS - 1) / KEYS * a.hkv, tiles = a.total_q * (a.hq / a.hkv) / used / (a.nseq > 0 ? a.nseq : 1);
+  const long n = blocks > 0 ? min(1024 / blocks, tiles / 8) : 1;
+  return (int)(n < 1 ? 1 : n > 8 ? 8 : n);
+}
+size_t delta_bytes(const hv_attn_packed_args& a) { return ((size_t)a.total_q * a.hq * sizeof(float) + 63) / 64 * 64; }
+
 template <typename T, int DP>
-void launch_backward(const Args& a, unsigned bq, unsigned bk, float* delta, hipStream_t s) {
+void launch_backward(const Args& a, unsigned bq, unsigned bk, hipStream_t s) {
+  float* delta = (float*)a.work;
+  float* part = (float*)((char*)a.work + delta_bytes(a));
+  const int parts = row_parts(a);
   if (a.total_q) {
     k_attn_packed_delta<T><<<(unsigned)min((a.total_q * a.hq + 15) / 16, 1L << 20), NT, 0, s>>>(a, delta);
     if (a.dq) k_attn_packed_dq<T, DP><<<bq, NT, 0, s>>>(a, delta);
   }
-  if (a.total_k && a.dk) k_attn_packed_dkv<T, DP><<<bk, NT, 0, s>>>(a, delta);
+  if (a.total_k && a.dk) {
+    k_attn_packed_dkv<T, DP><<<dim3(bk, parts), NT, 0, s>>>(a, delta, parts > 1 ? part : nullptr);
+    if (parts > 1)
+      k_attn_packed_sum<T><<<(unsigned)min((2 * a.total_k * a.hkv * a.d / 8 + NT - 1) / NT, 4096L), NT, 0, s>>>(a, parts, part);
+  }
 }
 
 // the tile width for a head dimension: the next of 32 / 64 / 128
@@ -1090,7 +1146,9 @@ extern "C" int hv_attn_packed(const hv_attn_packed_args* a, hv_stream_t stream) 
 }
 
 extern "C" size_t hv_attn_packed_backward_work_bytes(const hv_attn_packed_args* a) {
-  return a == nullptr || a->total_q <= 0 || a->hq <= 0 ? 0 : (size_t)a->total_q * a->hq * sizeof(float);
+  if (check_shape(a) != HV_OK) return 0;
+  const int n = row_parts(*a);
+  return delta_bytes(*a) + (n > 1 ? (size_t)n * 2 * a->total_k * a->hkv * a->d * sizeof(float) : 0);
 }
 
 extern "C" int hv_attn_packed_backward(const hv_attn_packed_args* a, hv_stream_t stream) {
@@ -1102,11 +1160,14 @@ extern "C" int hv_attn_packed_backward(const hv_attn_packed_args* a, hv_stream_t
                      ((uintptr_t)a->dq & 15) || a->work == nullptr))
     return HV_EINVAL;
   if ((a->dk == nullptr) != (a->dv == nullptr) || ((uintptr_t)a->dk & 15) || ((uintptr_t)a->dv & 15)) return HV_EINVAL;
+  // a tile of 64 packed rows is addressed with 32-bit offsets
+  const long reach = max(a->q_row, a->do_row) * 64 + max(a->q_head, a->do_head) * 64;
+  if (reach >= (1L << 29)) return HV_EUNSUPPORTED;
   const long bq = tile_bound(a->total_q, a->nseq, a->hq / a->hkv, 128) * a->hkv;
   const long bk = tile_bound(a->total_k, a->nseq, 1, KEYS) * a->hkv;
   if (bq >= MAX_BLOCKS || bk >= MAX_BLOCKS) return HV_EUNSUPPORTED;
   hipStream_t s = (hipStream_t)stream;
-  HV_DISPATCH(a->dtype, HV_HEAD_DIM(a->d, launch_backward, Args(*a), (unsigned)bq, (unsigned)bk, (float*)a->work, s));
+  HV_DISPATCH(a->dtype, HV_HEAD_DIM(a->d, launch_backward, Args(*a), (unsigned)bq, (unsigned)bk, s));
   HV_CHECK_LAUNCH();
   hv_diag_count(HV_KF_ATTN_PACKED);
   return HV_OK;

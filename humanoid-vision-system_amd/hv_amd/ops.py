@@ -843,8 +843,9 @@ def attn_packed_args(q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Tensor
                          f"v {tuple(v.shape)} {v.dtype} disagree")
     if hkv == 0 or hq == 0 or hq % hkv:
         raise ValueError(f"attention_packed: {hq} query heads do not share {hkv} key / value heads")
-    if d == 0 or d % 8 or d > 128 or hq > 1024:
-        raise ValueError(f"attention_packed: head dim {d} (a multiple of 8 up to 128), {hq} heads (up to 1024)")
+    if d == 0 or d % 8 or d > 128 or hq > 1024 or hq // hkv > 64:
+        raise ValueError(f"attention_packed: head dim {d} (a multiple of 8 up to 128), {hq} heads (up to 1024, and 64 per "
+                         f"key / value head) on {hkv}")
     if cu_q.dtype != torch.int32 or cu_k.dtype != torch.int32 or cu_q.dim() != 1 or cu_q.shape != cu_k.shape or \
             cu_q.numel() == 0 or not cu_q.is_contiguous() or not cu_k.is_contiguous():
         raise ValueError("attention_packed: cu_q and cu_k are int32 offsets [sequences + 1]")
@@ -871,7 +872,7 @@ def attention_packed(q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Option
     """softmax(scale q k^T) v over packed sequences of different lengths.
 
     q [rows, heads, d], k / v [rows, kv heads, d] (bf16 or fp32; rows and heads may lie apart), heads a
-    multiple of kv heads (query head h reads kv head h * kv heads // heads).  Sequence s owns the query rows
+    multiple of kv heads up to 64 times (query head h reads kv head h * kv heads // heads).  Sequence s owns the query rows
     cu_q[s] .. cu_q[s+1]-1 and the key rows cu_k[s] .. cu_k[s+1]-1 (int32 on the device, ascending; cu_k
     defaults to cu_q).  causal: query i of a sequence sees its keys up to i + (keys - queries), so one new
     token against a history is a sequence of one query.  scale defaults to d ** -0.5.

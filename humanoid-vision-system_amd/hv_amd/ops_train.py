@@ -509,9 +509,10 @@ def attention_packed_backward(q, k, v, cu_q, cu_k, causal: bool, scale: Optional
     """(dq, dk, dv) of attention_packed_train, dense; the ones that are not needed are None."""
     if dout.shape != q.shape or dout.dtype != q.dtype:
         raise ValueError(f"attention_packed_backward: dout {tuple(dout.shape)} {dout.dtype} is not like q")
+    # the kernels address 64 rows of q and dout with 32-bit offsets
+    q, dout = (t.contiguous() if t.numel() and not (rows_dense(t) and max(t.stride(0), t.stride(1)) < 1 << 22) else t
+               for t in (q, dout))
     a = attn_packed_args(q, k, v, cu_q, cu_k, causal, scale)
-    if dout.numel() and not rows_dense(dout):
-        dout = dout.contiguous()
     dq = torch.empty(q.shape, device=q.device, dtype=q.dtype) if need_q else None
     dk = torch.empty(k.shape, device=q.device, dtype=q.dtype) if need_kv else None
     dv = torch.empty(v.shape, device=q.device, dtype=q.dtype) if need_kv else None
