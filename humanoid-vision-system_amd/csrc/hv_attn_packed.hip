@@ -849,17 +849,19 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) k_att
 // waves 0 and 2 own the first 32 keys, 1 and 3 the others; 0 and 1 take a tile's first 32 rows, 2 and 3 the others, and
 // the two halves are added through LDS at the end.  (A block of 128 keys whose waves all walk over every row has the same
 // LDS traffic and half as many, twice as long blocks: 4096 + 2991 causal tokens, 4 heads, 760 against 700 us.)  Where the
-// keys give few blocks, gridDim.y blocks share a key tile's rows and write fp32 parts that k_attn_packed_sum adds in order.
+// keys give few blocks, `parts` blocks share a key tile's rows and write fp32 parts that k_attn_packed_sum adds in order.
 template <typename T, int DP>
 __global__ void __launch_bounds__(NT, DP * sizeof(T) >= 256 ? 1 : 2) k_attn_packed_dkv(const Args a, const float* __restrict__ delta,
-                                                                                          float* __restrict__ part_dk) {
+                                                                                          float* __restrict__ part_dk,
+                                                                                          int parts) {
   using L = Lay<T, DP>;
   auto fence = [] { if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0); };
   constexpr int BK = KEYS, BR = 64, TB = BR * L::ROWB;
   __shared__ __align__(16) char smem[4 * TB];          // Q and dO, two buffers
   __shared__ __align__(16) float st[2][2][BR];         // -lse log2 e and delta of the rows
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-  const int G = a.group.d, block = a.heads.div(blockIdx.x), kvh = a.heads.mod(blockIdx.x, block);
+  const int part = blockIdx.x % parts, x = blockIdx.x / parts;          // a tile's parts side by side: long blocks first
+  const int G = a.group.d, block = a.heads.div(x), kvh = a.heads.mod(x, block);
   const Tile t = find_tile(a.cu_k, a.nseq, a.total_k, 1, BK, block, false);
   if (t.seq < 0) return;
   int q0, lq;
@@ -905,8 +907,7 @@ __global__ void __launch_bounds__(NT, DP * sizeof(T) >= 256 ? 1 : 2) k_attn_pack
     }
   };
   // from the last rows, which every block of the sequence needs, backwards: blocks that run together read the same tiles
-  int tile = tn - 1 - (int)blockIdx.y;
-  const int parts = gridDim.y;
+  int tile = tn - 1 - part;
   if (tile >= t0) {
     sq.last(a.q_row, a.q_head, tile * used, rows, a.d, a.group, lds0);
     sg.last(a.do_row, a.do_head, tile * used, rows, a.d, a.group, lds0 + TB);
@@ -1004,8 +1005,8 @@ __global__ void __launch_bounds__(NT, DP * sizeof(T) >= 256 ? 1 : 2) k_attn_pack
     store_row<T, DP>((T*)a.dk + at, a.d, h, dk, a.scale);
   } else {
     const long all = a.total_k * a.heads.d * a.d;
-    store_row<float, DP>(part_dk + (2 * blockIdx.y) * all + at, a.d, h, dk, a.scale);
-    store_row<float, DP>(part_dk + (2 * blockIdx.y + 1) * all + at, a.d, h, dv, 1.f);
+    store_row<float, DP>(part_dk + (2 * part) * all + at, a.d, h, dk, a.scale);
+    store_row<float, DP>(part_dk + (2 * part + 1) * all + at, a.d, h, dv, 1.f);
   }
 }
 
@@ -1101,7 +1102,7 @@ void launch_backward(const Args& a, unsigned bq, unsigned bk, hipStream_t s) {
     if (a.dq) k_attn_packed_dq<T, DP><<<bq, NT, 0, s>>>(a, delta);
   }
   if (a.total_k && a.dk) {
-    k_attn_packed_dkv<T, DP><<<dim3(bk, parts), NT, 0, s>>>(a, delta, parts > 1 ? part : nullptr);
+    k_attn_packed_dkv<T, DP><<<bk * parts, NT, 0, s>>>(a, delta, parts > 1 ? part : nullptr, parts);
     if (parts > 1)
       k_attn_packed_sum<T><<<(unsigned)min((2 * a.total_k * a.hkv * a.d / 8 + NT - 1) / NT, 4096L), NT, 0, s>>>(a, parts, part);
   }
@@ -1165,7 +1166,7 @@ extern "C" int hv_attn_packed_backward(const hv_attn_packed_args* a, hv_stream_t
   if (reach >= (1L << 29)) return HV_EUNSUPPORTED;
   const long bq = tile_bound(a->total_q, a->nseq, a->hq / a->hkv, 128) * a->hkv;
   const long bk = tile_bound(a->total_k, a->nseq, 1, KEYS) * a->hkv;
-  if (bq >= MAX_BLOCKS || bk >= MAX_BLOCKS) return HV_EUNSUPPORTED;
+  if (bq >= MAX_BLOCKS || bk >= MAX_BLOCKS / 8) return HV_EUNSUPPORTED;
   hipStream_t s = (hipStream_t)stream;
   HV_DISPATCH(a->dtype, HV_HEAD_DIM(a->d, launch_backward, Args(*a), (unsigned)bq, (unsigned)bk, s));
   HV_CHECK_LAUNCH();
