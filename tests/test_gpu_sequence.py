@@ -524,6 +524,8 @@ def test_linear_fp8(gpu_device, m, n, k, out_dtype):
             pre = A @ W.t() + (0 if bias is None else bias.double().cpu())
             want = ACTS[act](pre)
             err = 1.13 * (loss + 4 * E * pre.abs()) + (2.0 ** -20 * (1 + pre.abs()) if act != "none" else 0)
+            if act == "gelu" and out_dtype == BF:                  # bf16 layers take the fitted GELU, 2.6e-5 at most off the
+                err = err + 2.7e-5                                 # erf form (minimax fit, csrc/hv_common.h hv_gelu_fast)
             got = ops.linear_fp8(a, sa, w, sw, bias=bias, act=act, out_dtype=out_dtype)
             assert got.dtype == out_dtype
             check(got, want, err + unit(out_dtype) * (want.abs() + err), (act, bias is None))
