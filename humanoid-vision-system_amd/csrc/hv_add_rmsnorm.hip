@@ -273,19 +273,26 @@ __global__ void __launch_bounds__(threads_of<TPR>()) k_add_rmsnorm_back(const No
     if (in(i)) store_vec<VW>(a.part + (long)blockIdx.x * a.cols + (t + i * TPR) * VW, dw[i]);
 }
 
-// dw[c] = sum_b part[b, c]: 32 columns x 32 shares of the blocks per workgroup
+// dw[c] = sum_b part[b, c]: 16 columns x 64 shares of the blocks per workgroup
 __global__ void __launch_bounds__(1024) k_norm_dw(const float* __restrict__ part, int nb, int cols, float* __restrict__ dw) {
-  __shared__ float red[32][33];
-  const int cl = threadIdx.x & 31, share = threadIdx.x >> 5, c = blockIdx.x * 32 + cl;
+  __shared__ float red[64][17];
+  const int cl = threadIdx.x & 15, share = threadIdx.x >> 4, c = blockIdx.x * 16 + cl;
   float v = 0.f;
-  if (c < cols)
-    for (int b = share; b < nb; b += 32) v += part[(long)b * cols + c];
+  if (c < cols) {
+#pragma unroll 4
+    for (int b = share; b < nb; b += 64) v += part[(long)b * cols + c];
+  }
   red[share][cl] = v;
+  __syncthreads();
+  if (share < 16) {
+    v = red[share][cl] + red[share + 16][cl] + red[share + 32][cl] + red[share + 48][cl];
+    red[share][cl] = v;                                   // read and written by this thread only
+  }
   __syncthreads();
   if (share == 0 && c < cols) {
     v = 0.f;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v += red[i][cl];
+    for (int i = 0; i < 16; ++i) v += red[i][cl];
     dw[c] = v;
   }
 }
@@ -379,7 +386,7 @@ extern "C" int hv_add_rmsnorm_backward(int r_dtype, const void* sum, const float
     HV_ROW_SHAPE(cols, wide, HV_NORM_CALL);
 #undef HV_NORM_CALL
   }
-  k_norm_dw<<<hv_cdiv(cols, 32), 1024, 0, s>>>(work, nb, cols, dscale);
+  k_norm_dw<<<hv_cdiv(cols, 16), 1024, 0, s>>>(work, nb, cols, dscale);
   HV_CHECK_LAUNCH();
   hv_diag_count(HV_KF_ADD_RMSNORM);
   return HV_OK;

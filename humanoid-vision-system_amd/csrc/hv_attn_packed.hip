@@ -386,11 +386,13 @@ __device__ __forceinline__ f32x16 zero16() {
 }
 
 // ------------------------------------------------------------------------------------------------
-// Forward: 4 waves of 32 packed rows each over tiles of BN keys that the block stages once.
-template <typename T, int DP, bool TRAIN>
-__global__ void __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) k_attn_packed(const Args a) {
+// Forward: 4 waves of 32 packed rows each over tiles of BN keys that the block stages once.  KS > 1, where the rows give
+// few blocks: KS waves share 32 rows, wave ks takes every KS-th run of BN keys (a tile is KS runs), and their sums are
+// joined through LDS in order.
+template <typename T, int DP, bool TRAIN, int KS>
+__global__ void __launch_bounds__(NT, DP * sizeof(T) * KS > 256 ? 1 : 2) k_attn_packed(const Args a) {
   using L = Lay<T, DP>;
-  constexpr int BM = 128, BN = L::ROWB > 256 ? 32 : 64, TB = BN * L::ROWB, NJ = BN / 32;
+  constexpr int BM = 128 / KS, BN = L::ROWB > 256 ? 32 : 64, BT = BN * KS, TB = BT * L::ROWB, NJ = BN / 32;
   __shared__ __align__(16) char smem[4 * TB];          // K and V, two buffers
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
   const int G = a.group.d, block = a.heads.div(blockIdx.x), kvh = a.heads.mod(blockIdx.x, block);
@@ -399,7 +401,7 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) k_att
   int k0, lk;
   seq_rows(a.cu_k, a.nseq, a.total_k, t.seq, k0, lk);
 
-  const int r = t.tile * BM + wave * 32 + (lane & 31);
+  const int ks = wave % KS, r = t.tile * BM + wave / KS * 32 + (lane & 31);
   const bool real = r < t.len * G;
   const int tok = real ? a.group.div(r) : 0, g = real ? a.group.mod(r, tok) : 0;
   const int late = lk - t.len;                           // the last query sees every key
@@ -430,10 +432,10 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) k_att
   float m = NEG_INF, l = 0.f, lt = 0.f;                  // running maximum, sum of rounded / of exact weights
   const float c2 = a.scale * LOG2E;
   const View<T, DP> view(lane);
-  const int ntile = (lim_blk + BN) / BN;
+  const int ntile = (lim_blk + BT) / BT;
 
   const unsigned lds0 = lds_at(smem);
-  KeyTiles<T, DP, BN> sk(kp, a.k_row, lim_blk + 1, a.d), sv(vp, a.v_row, lim_blk + 1, a.d);
+  KeyTiles<T, DP, BT> sk(kp, a.k_row, lim_blk + 1, a.d), sv(vp, a.v_row, lim_blk + 1, a.d);
   auto fetch = [&](int kt) {
     const unsigned at = lds0 + (kt & 1) * 2 * TB;
     sk.next(kt, at);
@@ -443,10 +445,11 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) k_att
   for (int kt = 0; kt < ntile; ++kt) {
     arrived();
     __syncthreads();                                     // tile kt is here, the other buffer is no longer read
-    const char* tk = smem + (kt & 1) * 2 * TB;
+    const char* tk = smem + (kt & 1) * 2 * TB + ks * BN * L::ROWB;
     const char* tv = tk + TB;
     if (kt + 1 < ntile) fetch(kt + 1);
-    if (kt * BN > lim_hi) continue;
+    const int key = kt * BT + ks * BN;                   // this wave's first key of the tile
+    if (key > lim_hi) continue;
     f32x16 s[NJ];
 #pragma unroll
     for (int j = 0; j < NJ; ++j) s[j] = zero16();
@@ -455,12 +458,12 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) k_att
 #pragma unroll
       for (int j = 0; j < NJ; ++j) s[j] = mma16(view.rows(tk + j * 32 * L::ROWB, i), q[i], s[j]);
     }
-    if (kt * BN + BN - 1 > lim_lo) {
+    if (key + BN - 1 > lim_lo) {
 #pragma unroll
       for (int j = 0; j < NJ; ++j)
 #pragma unroll
         for (int x = 0; x < 16; ++x)
-          if (kt * BN + 32 * j + 8 * (x >> 2) + 4 * h + (x & 3) > lim) s[j][x] = NEG_INF;
+          if (key + 32 * j + 8 * (x >> 2) + 4 * h + (x & 3) > lim) s[j][x] = NEG_INF;
     }
     float top = s[0][0];
 #pragma unroll
@@ -505,9 +508,49 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) k_att
           o[dt] = mma16(view.cols(tv + (32 * j + 16 * i) * L::ROWB, dt), p, o[dt]);
       }
   }
-  if (!real) return;
   l += other_half(l);
   if constexpr (TRAIN && sizeof(T) == 2) lt += other_half(lt); else lt = l;
+  if constexpr (KS > 1) {                                // wave ks = 0 joins its rows' sums
+    constexpr int W = 16 * L::NDT + 3;
+    float* part = (float*)smem + (wave / KS * (KS - 1) + ks - 1) * W * 64 + lane;
+    static_assert(4 / KS * (KS - 1) * W * 64 * 4 <= 4 * TB, "the joined sums fit the tiles' LDS");
+    __syncthreads();
+    if (ks > 0) {
+      part[0] = m;
+      part[64] = l;
+      part[128] = lt;
+#pragma unroll
+      for (int i = 0; i < L::NDT; ++i)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) part[(3 + i * 16 + x) * 64] = o[i][x];
+    }
+    __syncthreads();
+    if (ks > 0) return;
+    float mx = m;
+    part += W * 64;                                      // of ks = 1
+#pragma unroll
+    for (int k = 0; k < KS - 1; ++k) mx = fmaxf(mx, part[k * W * 64]);
+    const float f0 = m == NEG_INF ? 1.f : __builtin_amdgcn_exp2f((m - mx) * c2);
+    l *= f0;
+    lt *= f0;
+#pragma unroll
+    for (int i = 0; i < L::NDT; ++i)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) o[i][x] *= f0;
+#pragma unroll
+    for (int k = 0; k < KS - 1; ++k) {
+      const float* pk = part + k * W * 64;
+      const float f = pk[0] == NEG_INF ? 1.f : __builtin_amdgcn_exp2f((pk[0] - mx) * c2);
+      l = fmaf(pk[64], f, l);
+      lt = fmaf(pk[128], f, lt);
+#pragma unroll
+      for (int i = 0; i < L::NDT; ++i)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) o[i][x] = fmaf(pk[(3 + i * 16 + x) * 64], f, o[i][x]);
+    }
+    m = mx;
+  }
+  if (!real) return;
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
   const long orow = (qrow * a.hq + qh) * a.d;
   store_row<T, DP>((T*)a.out + orow, a.d, h, o, inv);
@@ -755,11 +798,11 @@ __global__ void __launch_bounds__(NT) k_attn_packed_delta(const Args a, float* _
   }
 }
 
-// dQ: the forward's walk over the keys with dO beside Q; dQ^T += K^T dS^T
-template <typename T, int DP>
-__global__ void __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) k_attn_packed_dq(const Args a, const float* __restrict__ delta) {
+// dQ: the forward's walk over the keys with dO beside Q; dQ^T += K^T dS^T.  KS: as in the forward
+template <typename T, int DP, int KS>
+__global__ void __launch_bounds__(NT, DP * sizeof(T) * KS > 256 ? 1 : 2) k_attn_packed_dq(const Args a, const float* __restrict__ delta) {
   using L = Lay<T, DP>;
-  constexpr int BM = 128, BN = L::ROWB > 256 ? 32 : 64, TB = BN * L::ROWB;
+  constexpr int BM = 128 / KS, BN = L::ROWB > 256 ? 32 : 64, BT = BN * KS, TB = BT * L::ROWB;
   __shared__ __align__(16) char smem[4 * TB];          // K and V, two buffers
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
   const int G = a.group.d, block = a.heads.div(blockIdx.x), kvh = a.heads.mod(blockIdx.x, block);
@@ -767,7 +810,7 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) k_att
   if (t.seq < 0) return;
   int k0, lk;
   seq_rows(a.cu_k, a.nseq, a.total_k, t.seq, k0, lk);
-  const int r = t.tile * BM + wave * 32 + (lane & 31);
+  const int ks = wave % KS, r = t.tile * BM + wave / KS * 32 + (lane & 31);
   const bool real = r < t.len * G;
   const int tok = real ? a.group.div(r) : 0, g = real ? a.group.mod(r, tok) : 0;
   const int late = lk - t.len;
@@ -801,9 +844,9 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) k_att
 #pragma unroll
   for (int i = 0; i < L::NDT; ++i) dq[i] = zero16();
   const View<T, DP> view(lane);
-  const int ntile = (lim_blk + BN) / BN;
+  const int ntile = (lim_blk + BT) / BT;
   const unsigned lds0 = lds_at(smem);
-  KeyTiles<T, DP, BN> sk(kp, a.k_row, lim_blk + 1, a.d), sv(vp, a.v_row, lim_blk + 1, a.d);
+  KeyTiles<T, DP, BT> sk(kp, a.k_row, lim_blk + 1, a.d), sv(vp, a.v_row, lim_blk + 1, a.d);
   auto fetch = [&](int kt) {
     const unsigned at = lds0 + (kt & 1) * 2 * TB;
     sk.next(kt, at);
@@ -813,12 +856,12 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) k_att
   for (int kt = 0; kt < ntile; ++kt) {
     arrived();
     __syncthreads();                                     // tile kt is here, the other buffer is no longer read
-    const char* tk = smem + (kt & 1) * 2 * TB;
+    const char* tk = smem + (kt & 1) * 2 * TB + ks * BN * L::ROWB;
     const char* tv = tk + TB;
     if (kt + 1 < ntile) fetch(kt + 1);
 #pragma unroll 1
     for (int j = 0; j < BN / 32; ++j) {
-      const int key = kt * BN + 32 * j;
+      const int key = kt * BT + ks * BN + 32 * j;
       if (key > lim_hi) break;
       f32x16 s = zero16(), dp = zero16();
 #pragma unroll
@@ -841,6 +884,23 @@ __global__ void __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) k_att
           dq[dt] = mma16(view.cols(tk + (32 * j + 16 * i) * L::ROWB, dt), p, dq[dt]);
       }
     }
+  }
+  if constexpr (KS > 1) {
+    static_assert(KS == 2 && 2 * 16 * L::NDT * 64 * 4 <= 4 * TB, "the second wave's sums fit the tiles' LDS");
+    float* half = (float*)smem + wave / KS * 16 * L::NDT * 64 + lane;
+    __syncthreads();
+    if (ks == 1) {
+#pragma unroll
+      for (int i = 0; i < L::NDT; ++i)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) half[(i * 16 + x) * 64] = dq[i][x];
+    }
+    __syncthreads();
+    if (ks == 1) return;
+#pragma unroll
+    for (int i = 0; i < L::NDT; ++i)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) dq[i][x] += half[(i * 16 + x) * 64];
   }
   if (real) store_row<T, DP>((T*)a.dq + (qrow * a.hq + qh) * a.d, a.d, h, dq, a.scale);
 }
@@ -1078,9 +1138,21 @@ template <typename T, int DP> void launch_keys(const Args& a, int n, hipStream_t
   k_attn_packed_join<T><<<hv_cdiv(a.total_q * a.hq, 4), NT, 0, s>>>(a, n, po, pml);
 }
 
-template <typename T, int DP> void launch_forward(const Args& a, unsigned blocks, hipStream_t s) {
-  if (a.lse != nullptr || a.out_low != nullptr) k_attn_packed<T, DP, true><<<blocks, NT, 0, s>>>(a);
-  else k_attn_packed<T, DP, false><<<blocks, NT, 0, s>>>(a);
+// Waves that share 32 rows of the forward's tile form: two where blocks of 128 rows would not give every CU two.  (4269 image
+// tokens, 8 heads of 32, 272 such blocks: KS 1 / 2 / 4 take 24.9 / 16.7 / 22.4 us; 8569 tokens, 16 heads of 64 on 4, 1076
+// blocks: 88.7 / 97.1 us.)
+int key_split(const hv_attn_packed_args& a) {
+  return (a.total_q * (a.hq / a.hkv) + 127) / 128 * a.hkv < 512 ? 2 : 1;
+}
+
+template <typename T, int DP, int KS> void launch_forward_ks(const Args& a, hipStream_t s) {
+  const unsigned blocks = (unsigned)(tile_bound(a.total_q, a.nseq, a.group.d, 128 / KS) * a.hkv);
+  if (a.lse != nullptr || a.out_low != nullptr) k_attn_packed<T, DP, true, KS><<<blocks, NT, 0, s>>>(a);
+  else k_attn_packed<T, DP, false, KS><<<blocks, NT, 0, s>>>(a);
+}
+template <typename T, int DP> void launch_forward(const Args& a, hipStream_t s) {
+  if (key_split(a) == 1) launch_forward_ks<T, DP, 1>(a, s);
+  else launch_forward_ks<T, DP, 2>(a, s);
 }
 
 // Blocks that share the rows of a key tile (see k_attn_packed_dkv): up to four blocks per CU, eight row tiles each at least
@@ -1093,13 +1165,16 @@ int row_parts(const hv_attn_packed_args& a) {
 size_t delta_bytes(const hv_attn_packed_args& a) { return ((size_t)a.total_q * a.hq * sizeof(float) + 63) / 64 * 64; }
 
 template <typename T, int DP>
-void launch_backward(const Args& a, unsigned bq, unsigned bk, hipStream_t s) {
+void launch_backward(const Args& a, unsigned bk, hipStream_t s) {
   float* delta = (float*)a.work;
   float* part = (float*)((char*)a.work + delta_bytes(a));
   const int parts = row_parts(a);
   if (a.total_q) {
     k_attn_packed_delta<T><<<(unsigned)min((a.total_q * a.hq + 15) / 16, 1L << 20), NT, 0, s>>>(a, delta);
-    if (a.dq) k_attn_packed_dq<T, DP><<<bq, NT, 0, s>>>(a, delta);
+    if (a.dq && key_split(a) == 1)
+      k_attn_packed_dq<T, DP, 1><<<(unsigned)(tile_bound(a.total_q, a.nseq, a.group.d, 128) * a.hkv), NT, 0, s>>>(a, delta);
+    else if (a.dq)
+      k_attn_packed_dq<T, DP, 2><<<(unsigned)(tile_bound(a.total_q, a.nseq, a.group.d, 64) * a.hkv), NT, 0, s>>>(a, delta);
   }
   if (a.total_k && a.dk) {
     k_attn_packed_dkv<T, DP><<<bk * parts, NT, 0, s>>>(a, delta, parts > 1 ? part : nullptr, parts);
@@ -1131,8 +1206,7 @@ extern "C" int hv_attn_packed(const hv_attn_packed_args* a, hv_stream_t stream) 
   if (rc != HV_OK) return rc;
   if (a->total_q == 0) return HV_OK;
   if (a->out == nullptr || ((uintptr_t)a->out & 15) || ((uintptr_t)a->out_low & 15)) return HV_EINVAL;
-  const long blocks = tile_bound(a->total_q, a->nseq, a->hq / a->hkv, 128) * a->hkv;
-  if (blocks >= MAX_BLOCKS) return HV_EUNSUPPORTED;
+  if (tile_bound(a->total_q, a->nseq, a->hq / a->hkv, 64) * a->hkv >= MAX_BLOCKS) return HV_EUNSUPPORTED;
   hipStream_t s = (hipStream_t)stream;
   const int n = part_keys(*a);
   if (n) {
@@ -1140,7 +1214,7 @@ extern "C" int hv_attn_packed(const hv_attn_packed_args* a, hv_stream_t stream) 
       return HV_EINVAL;
     HV_DISPATCH(a->dtype, HV_HEAD_DIM(a->d, launch_keys, Args(*a), n, s));
   } else
-    HV_DISPATCH(a->dtype, HV_HEAD_DIM(a->d, launch_forward, Args(*a), (unsigned)blocks, s));
+    HV_DISPATCH(a->dtype, HV_HEAD_DIM(a->d, launch_forward, Args(*a), s));
   HV_CHECK_LAUNCH();
   hv_diag_count(HV_KF_ATTN_PACKED);
   return HV_OK;
@@ -1164,11 +1238,11 @@ extern "C" int hv_attn_packed_backward(const hv_attn_packed_args* a, hv_stream_t
   // a tile of 64 packed rows is addressed with 32-bit offsets
   const long reach = max(a->q_row, a->do_row) * 64 + max(a->q_head, a->do_head) * 64;
   if (reach >= (1L << 29)) return HV_EUNSUPPORTED;
-  const long bq = tile_bound(a->total_q, a->nseq, a->hq / a->hkv, 128) * a->hkv;
+  const long bq = tile_bound(a->total_q, a->nseq, a->hq / a->hkv, 64) * a->hkv;
   const long bk = tile_bound(a->total_k, a->nseq, 1, KEYS) * a->hkv;
   if (bq >= MAX_BLOCKS || bk >= MAX_BLOCKS / 8) return HV_EUNSUPPORTED;
   hipStream_t s = (hipStream_t)stream;
-  HV_DISPATCH(a->dtype, HV_HEAD_DIM(a->d, launch_backward, Args(*a), (unsigned)bq, (unsigned)bk, s));
+  HV_DISPATCH(a->dtype, HV_HEAD_DIM(a->d, launch_backward, Args(*a), (unsigned)bk, s));
   HV_CHECK_LAUNCH();
   hv_diag_count(HV_KF_ATTN_PACKED);
   return HV_OK;
