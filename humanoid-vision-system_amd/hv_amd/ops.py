@@ -799,15 +799,17 @@ def attention_general(q: Tensor, k: Tensor, v: Tensor, heads: int, key_padding_m
 class on_device:
     """Launch on `t`'s device and its current stream, also where another device is the current one."""
 
+    __slots__ = ("index", "guard")
+
     def __init__(self, t: Tensor):
-        self.index = t.device.index
+        self.index = t.get_device()
         self.guard = None
 
     def __enter__(self):
         if self.index != torch.cuda.current_device():
             self.guard = torch.cuda.device(self.index)
             self.guard.__enter__()
-        return stream_ptr()
+        return torch._C._cuda_getCurrentRawStream(self.index)
 
     def __exit__(self, *exc):
         if self.guard is not None:
@@ -825,9 +827,8 @@ def _same_device(what: str, first: Tensor, *others) -> None:
 def rows_dense(t: Tensor) -> bool:
     """Whether attention_packed can read `t` [rows, heads, d] in place: last dimension dense, every row
     start on a 16-byte boundary."""
-    es = t.element_size()
-    return (t.stride(2) == 1 or t.shape[2] == 1) and t.data_ptr() % 16 == 0 and \
-        (t.stride(0) * es) % 16 == 0 and (t.stride(1) * es) % 16 == 0
+    row, head, one = t.stride()
+    return (one == 1 or t.shape[2] == 1) and not (t.data_ptr() | row * t.element_size() | head * t.element_size()) & 15
 
 
 def attn_packed_args(q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Tensor, causal: bool,
@@ -836,9 +837,9 @@ def attn_packed_args(q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Tensor
     _same_device("attention_packed", q, k, v, cu_q, cu_k)
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise ValueError("attention_packed: q is [rows, heads, d], k and v are [rows, kv heads, d]")
-    hq, d = q.shape[1], q.shape[2]
-    hkv = k.shape[1]
-    if k.shape != v.shape or k.shape[2] != d or q.dtype != k.dtype or q.dtype != v.dtype:
+    tq, hq, d = q.shape
+    tk, hkv, dk = k.shape
+    if k.shape != v.shape or dk != d or q.dtype != k.dtype or q.dtype != v.dtype:
         raise ValueError(f"attention_packed: q {tuple(q.shape)} {q.dtype}, k {tuple(k.shape)} {k.dtype}, "
                          f"v {tuple(v.shape)} {v.dtype} disagree")
     if hkv == 0 or hq == 0 or hq % hkv:
@@ -850,21 +851,24 @@ def attn_packed_args(q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Tensor
             cu_q.numel() == 0 or not cu_q.is_contiguous() or not cu_k.is_contiguous():
         raise ValueError("attention_packed: cu_q and cu_k are int32 offsets [sequences + 1]")
     for name, t in (("q", q), ("k", k), ("v", v)):
-        if t.numel() and not rows_dense(t):
+        if not rows_dense(t) and t.numel():
             raise ValueError(f"attention_packed: {name} needs a dense last dimension and 16-byte aligned rows "
                              f"(strides {t.stride()})")
     scale = d ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < 3e38:
         raise ValueError(f"attention_packed: scale {scale} is not a positive finite number")
-    a = L.AttnPackedArgs()
-    a.dtype, a.hq, a.hkv, a.d, a.nseq, a.causal = dtype_code(q.dtype), hq, hkv, d, cu_q.numel() - 1, int(bool(causal))
-    a.scale, a.total_q, a.total_k = scale, q.shape[0], k.shape[0]
+    a = L.AttnPackedArgs(dtype_code(q.dtype), hq, hkv, d, cu_q.numel() - 1, bool(causal), scale, 0, tq, tk)
+    attn_packed_point(a, q, k, v, cu_q, cu_k)
+    return a
+
+
+def attn_packed_point(a: L.AttnPackedArgs, q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Tensor) -> None:
+    """Let the description of a call point at its operands."""
     a.cu_q, a.cu_k = cu_q.data_ptr(), cu_k.data_ptr()
     a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    a.q_row, a.q_head = q.stride(0), q.stride(1)
-    a.k_row, a.k_head = k.stride(0), k.stride(1)
-    a.v_row, a.v_head = v.stride(0), v.stride(1)
-    return a
+    a.q_row, a.q_head, _ = q.stride()
+    a.k_row, a.k_head, _ = k.stride()
+    a.v_row, a.v_head, _ = v.stride()
 
 
 def attention_packed(q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Optional[Tensor] = None, *,

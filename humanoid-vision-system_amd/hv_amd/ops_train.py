@@ -14,7 +14,7 @@ from torch.autograd.graph import increment_version
 
 from . import _lib as L
 from ._lib import check, dtype_code, ptr, stream_ptr
-from .ops import _contig, _cuda, attn_packed_args, f32, norm_operands, on_device, rows_dense
+from .ops import _contig, _cuda, attn_packed_args, attn_packed_point, f32, norm_operands, on_device, rows_dense
 from .runtime import options, seed_offset_ptr
 
 Tensor = torch.Tensor
@@ -487,9 +487,9 @@ def attention_backward(q, k, v, o, do, lse, heads: int, drop_p: float, seed: int
 
 def attention_packed_train(q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Tensor, causal: bool,
                            scale: Optional[float]):
-    """ops.attention_packed with what its backward needs: (out, out_low, lse).  out_low (bf16 only) is the part
-    of out that its rounding cut off: the backward's row mean dO . O would otherwise carry that rounding into
-    every score gradient of the row."""
+    """ops.attention_packed with what its backward needs: (out, out_low, lse, call).  out_low (bf16 only) is the
+    part of out that its rounding cut off: the backward's row mean dO . O would otherwise carry that rounding into
+    every score gradient of the row.  call: the checked description of the operands."""
     a = attn_packed_args(q, k, v, cu_q, cu_k, causal, scale)
     out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
     low = torch.empty_like(out) if q.dtype == torch.bfloat16 else None
@@ -501,25 +501,27 @@ def attention_packed_train(q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: 
         work = torch.empty(n, device=q.device, dtype=torch.uint8) if n else None
         a.work = ptr(work)
         check(lib.hv_attn_packed(C.byref(a), stream), "hv_attn_packed")
-    return out, low, lse
+    return out, low, lse, a
 
 
-def attention_packed_backward(q, k, v, cu_q, cu_k, causal: bool, scale: Optional[float], out, low, lse, dout,
-                              need_q: bool = True, need_kv: bool = True):
+def attention_packed_backward(q, k, v, cu_q, cu_k, call, out, low, lse, dout, need_q: bool = True,
+                              need_kv: bool = True):
     """(dq, dk, dv) of attention_packed_train, dense; the ones that are not needed are None."""
     if dout.shape != q.shape or dout.dtype != q.dtype:
         raise ValueError(f"attention_packed_backward: dout {tuple(dout.shape)} {dout.dtype} is not like q")
     # the kernels address 64 rows of q and dout with 32-bit offsets
-    q, dout = (t.contiguous() if t.numel() and not (rows_dense(t) and max(t.stride(0), t.stride(1)) < 1 << 22) else t
+    q, dout = (t.contiguous() if not (rows_dense(t) and max(t.stride()) < 1 << 22) and t.numel() else t
                for t in (q, dout))
-    a = attn_packed_args(q, k, v, cu_q, cu_k, causal, scale)
+    a = L.AttnPackedArgs.from_buffer_copy(call)
+    attn_packed_point(a, q, k, v, cu_q, cu_k)
     dq = torch.empty(q.shape, device=q.device, dtype=q.dtype) if need_q else None
     dk = torch.empty(k.shape, device=q.device, dtype=q.dtype) if need_kv else None
     dv = torch.empty(v.shape, device=q.device, dtype=q.dtype) if need_kv else None
     lib = L.lib()
     with on_device(q) as stream:
         a.out, a.out_low, a.lse = out.data_ptr(), ptr(low), lse.data_ptr()
-        a.dout, a.do_row, a.do_head = dout.data_ptr(), dout.stride(0), dout.stride(1)
+        a.dout = dout.data_ptr()
+        a.do_row, a.do_head, _ = dout.stride()
         a.dq, a.dk, a.dv = ptr(dq), ptr(dk), ptr(dv)
         work = torch.empty(lib.hv_attn_packed_backward_work_bytes(C.byref(a)), device=q.device, dtype=torch.uint8)
         a.work = work.data_ptr()

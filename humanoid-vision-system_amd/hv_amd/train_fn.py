@@ -480,8 +480,7 @@ class PackedAttentionFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k, causal: bool, scale):
-        out, low, lse = T.attention_packed_train(q, k, v, cu_q, cu_k, causal, scale)
-        ctx.meta = (causal, scale)
+        out, low, lse, ctx.call = T.attention_packed_train(q, k, v, cu_q, cu_k, causal, scale)
         ctx.save_for_backward(q, k, v, cu_q, cu_k, out, low, lse)
         return out
 
@@ -489,7 +488,7 @@ class PackedAttentionFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, g):
         q, k, v, cu_q, cu_k, out, low, lse = ctx.saved_tensors
-        dq, dk, dv = T.attention_packed_backward(q, k, v, cu_q, cu_k, *ctx.meta, out, low, lse, g, _need(ctx, 0),
+        dq, dk, dv = T.attention_packed_backward(q, k, v, cu_q, cu_k, ctx.call, out, low, lse, g, _need(ctx, 0),
                                                  _need(ctx, 1) or _need(ctx, 2))
         return dq, dk, dv, None, None, None, None
 
