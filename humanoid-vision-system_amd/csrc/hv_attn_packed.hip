@@ -1117,12 +1117,16 @@ constexpr long MAX_BLOCKS = 1L << 24;                    // a grid stays below 2
 // blocks that cover `total` rows in nseq sequences and the two ranges outside of them, BM packed rows each
 long tile_bound(long total, int nseq, int G, int BM) { return total * G / BM + nseq + 2; }
 
-// Keys of a part in the few-rows form, 0: the tile form.  Few rows: on average at most 64 packed rows per sequence (the
-// tile form would leave its second tile half empty and give one block all of a sequence's keys).  Parts are sized for
-// about four blocks per CU, 128 keys (one slab per wave) at least.
+// Keys of a part in the few-rows form, 0: the tile form.  The few-rows form reads a sequence's keys once per 32 of its rows
+// and needs a second launch; the tile form gives one block all the keys of 64 or 128 rows, 128 keys a step.  Averages per
+// sequence decide: few rows where there are 512 keys for it and for each 32 rows (at most 8 times).  Measured, tile / few
+// rows, us: 1 x 4 rows, 4096 keys of 128: 69 / 14; 8 x 4, 1024: 22 / 15; 64 x 4, 1024: 47 / 45; 8 x 64, 1024: 21 / 26; 1 x 64,
+// 4096: 59 / 22; 64 columns: 64 x 1, 512: 12 / 18; 8 x 64, 1024: 13 / 19; 1 x 128, 4096: 35 / 25.
+// Parts are sized for about four blocks per CU, 128 keys (one slab per wave) at least.
 int part_keys(const hv_attn_packed_args& a) {
-  const int G = a.hq / a.hkv;
-  if (a.nseq == 0 || a.total_q == 0 || a.total_k == 0 || a.total_q * G > 64L * a.nseq) return 0;
+  if (a.nseq == 0 || a.total_q == 0 || a.total_k == 0) return 0;
+  const long tiles = (a.total_q * (a.hq / a.hkv) + 32L * a.nseq - 1) / (32L * a.nseq);      // of 32 rows a sequence
+  if (tiles > 8 || a.total_k < 512 * (tiles + 1) * a.nseq) return 0;
   long n = (a.total_k * a.hkv + 1023) / 1024;
   n = (n + 127) / 128 * 128;
   return (int)(n < 128 ? 128 : n);

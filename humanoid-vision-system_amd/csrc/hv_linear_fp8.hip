@@ -127,9 +127,11 @@ __global__ void __launch_bounds__(512) k_linear_fp8_rows(const LinArgs p) {
 }
 
 // ------------------------------------------------------------------------------------------------
-// Tiles of 256 rows x 256 outputs, 8 waves of 128 outputs x 64 rows (2 along the outputs, 4 along the rows).  k goes by in
-// stages of 128 codes, a whole cache line of a row (stages of 64 fetch every line twice), two in LDS: one read, one on its way.
-constexpr int NT = 512, BM = 256, BN = 256, BK = 128, TILE = 256 * BK, STAGE = 2 * TILE;
+// Tiles.  A wave owns 32 NT_ outputs x 32 MT_ rows, a block WN x WM waves.  k goes by in stages of 128 codes, a whole cache
+// line of a row (stages of 64 fetch every line twice), STAGES of them in LDS: one read, the others on their way or free.
+// 256 x 256 with two stages (8 waves of 128 x 64) where such tiles fill the chip; 64 x 64 with six (4 waves of 32 x 32) where
+// they do not and the latency of the stages is what counts; 128 x 128 with three in between.
+constexpr int BK = 128;
 
 __device__ const uint4 zeros = {0, 0, 0, 0};              // what lies behind k
 
@@ -154,9 +156,12 @@ template <typename T> __device__ __forceinline__ T part(u32x4 v, int e) {
   else return __uint_as_float(v[e]);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(NT, 2) k_linear_fp8(const LinArgs p, int tiles_m, int tiles_n) {
-  __shared__ __align__(16) unsigned char sm[2 * STAGE];
+template <typename T, int WN, int WM, int NT_, int MT_, int STAGES>
+__global__ void __launch_bounds__(64 * WN * WM, WN * WM / 4) k_linear_fp8(const LinArgs p, int tiles_m, int tiles_n) {
+  constexpr int BM = 32 * MT_ * WM, BN = 32 * NT_ * WN, TN = BN * BK, STAGE = TN + BM * BK;
+  constexpr int WAVES = WN * WM, DN = BN / 8 / WAVES, DM = BM / 8 / WAVES, D = DN + DM;   // DMA instructions of a wave and stage
+  static_assert(DN * 8 * WAVES == BN && DM * 8 * WAVES == BM && (STAGES - 2) * D < 64, "whole instructions");
+  __shared__ __align__(16) unsigned char sm[STAGES * STAGE];
   __shared__ __align__(16) float col_scale[BN], col_bias[BN];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, r31 = lane & 31;
   // Blocks b = x mod 8 run on one XCD: it gets a run of tiles, in columns of 8 row tiles, whose a and w tiles share its L2
@@ -165,93 +170,96 @@ __global__ void __launch_bounds__(NT, 2) k_linear_fp8(const LinArgs p, int tiles
   const int band = id / (8 * tiles_n), in = id - band * 8 * tiles_n, high = min(8, tiles_m - band * 8);
   const long m0 = (long)(band * 8 + in % high) * BM;
   const int n0 = in / high * BN;
-  const int wn = (wave & 1) * 128, wm = (wave >> 1) * 64;
+  const int wn = wave % WN * 32 * NT_, wm = wave / WN * 32 * MT_;
 
-  // the wave's eight DMA instructions of a stage: rows (4 wave + i) 8 + lane / 8 of w (i = 0 .. 3) and of a
-  const unsigned char* src[8];
-  const int kc0 = lane & 7;
+  // the wave's DMA instructions of a stage: rows (DN wave + i) 8 + lane / 8 of w, then rows (DM wave + i) 8 + lane / 8 of a
+  auto place = [&](int i) { return i < DN ? (wave * DN + i) * 8 : (wave * DM + i - DN) * 8; };
+  const unsigned char* src[D];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int row = (wave * 4 + (i & 3)) * 8 + (lane >> 3);
-    src[i] = (i < 4 ? p.w + (long)min(n0 + row, p.n - 1) * p.ldw : p.a + min(m0 + row, p.m - 1) * p.lda) + (kc0 ^ swz(row)) * 16;
+  for (int i = 0; i < D; ++i) {
+    const int row = place(i) + (lane >> 3);
+    src[i] = (i < DN ? p.w + (long)min(n0 + row, p.n - 1) * p.ldw : p.a + min(m0 + row, p.m - 1) * p.lda) + ((lane & 7) ^ swz(row)) * 16;
   }
   const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)sm;
   const int stages = (p.k + BK - 1) / BK;
-  auto issue = [&](int s) {
-    const unsigned at = lds0 + (s & 1) * STAGE + wave * 4096;
-    if ((s + 1) * BK <= p.k) {
+  auto issue = [&](int s, int buf) {
+    const unsigned at = lds0 + buf * STAGE;
+    const bool whole = (s + 1) * BK <= p.k;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        dma16(src[i], at + (i >> 2) * TILE + (i & 3) * 1024);
+    for (int i = 0; i < D; ++i) {
+      const unsigned to = at + (i < DN ? 0 : TN) + place(i) * BK;
+      if (whole) {
+        dma16(src[i], to);
         src[i] += BK;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int row = (wave * 4 + (i & 3)) * 8 + (lane >> 3);
-        dma16(s * BK + (kc0 ^ swz(row)) * 16 < p.k ? (const void*)src[i] : (const void*)&zeros, at + (i >> 2) * TILE + (i & 3) * 1024);
+      } else {
+        dma16(s * BK + ((lane & 7) ^ swz(place(i) + (lane >> 3))) * 16 < p.k ? (const void*)src[i] : (const void*)&zeros, to);
       }
     }
   };
   // LDS offsets of the lane's operand rows (32-row tiles are 32 * BK apart and permuted alike); step 1 of a stage: ^ 64
   const int f = swz(r31);
   const int o0 = r31 * BK + (((2 * half) ^ f) << 4), o1 = r31 * BK + (((2 * half + 1) ^ f) << 4);
-  f32x16 acc[4][2];
+  f32x16 acc[NT_][MT_];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < NT_; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < MT_; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-  struct Ops { i32x8 w[4], a[2]; };
-  auto read = [&](Ops& o, int s, int ks) {
-    const unsigned char* tw = sm + (s & 1) * STAGE + wn * BK;
-    const unsigned char* ta = sm + (s & 1) * STAGE + TILE + wm * BK;
+  struct Ops { i32x8 w[NT_], a[MT_]; };
+  auto read = [&](Ops& o, const unsigned char* stage, int ks) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o.w[i] = operand(tw + i * 32 * BK, o0 ^ (ks << 6), o1 ^ (ks << 6));
+    for (int i = 0; i < NT_; ++i) o.w[i] = operand(stage + (wn + i * 32) * BK, o0 ^ (ks << 6), o1 ^ (ks << 6));
 #pragma unroll
-    for (int j = 0; j < 2; ++j) o.a[j] = operand(ta + j * 32 * BK, o0 ^ (ks << 6), o1 ^ (ks << 6));
+    for (int j = 0; j < MT_; ++j) o.a[j] = operand(stage + TN + (wm + j * 32) * BK, o0 ^ (ks << 6), o1 ^ (ks << 6));
   };
   auto multiply = [&](const Ops& o) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < NT_; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < MT_; ++j)
         acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(o.w[i], o.a[j], acc[i][j], 0, 0, 0, UNIT, 0, UNIT);
   };
   const bool live = m0 + wm < p.m && n0 + wn < p.n;        // whether this wave has outputs
-  if (threadIdx.x < BN) {
-    const int n = min(n0 + (int)threadIdx.x, p.n - 1);
-    col_scale[threadIdx.x] = p.ws[n];
-    col_bias[threadIdx.x] = p.bias ? p.bias[n] : 0.f;
+  for (int i = threadIdx.x; i < BN; i += 64 * WAVES) {
+    const int n = min(n0 + i, p.n - 1);
+    col_scale[i] = p.ws[n];
+    col_bias[i] = p.bias ? p.bias[n] : 0.f;
   }
-  issue(0);
-  for (int s = 0; s < stages; ++s) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();                                      // stage s is here, the other buffer is no longer read
-    if (s + 1 < stages) issue(s + 1);
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s)
+    if (s < stages) issue(s, s);
+  for (int s = 0, buf = 0; s < stages; ++s, buf = buf + 1 == STAGES ? 0 : buf + 1) {
+    // all but the newer stages' instructions of this wave have arrived; after the barrier: every wave's, and the buffer that
+    // the step before read is free
+    if (s + STAGES - 2 < stages) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 2) * D) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (s + STAGES - 1 < stages) issue(s + STAGES - 1, buf == 0 ? STAGES - 1 : buf - 1);
     if (!live) continue;
     Ops x, y;
-    read(x, s, 0);
-    read(y, s, 1);
+    read(x, sm + buf * STAGE, 0);
+    read(y, sm + buf * STAGE, 1);
     multiply(x);
     multiply(y);
   }
-  // out: the wave's 64 rows x 128 outputs through its own 16 KiB of LDS (bf16; fp32 in two halves), rows of 16-byte pieces
+  // out: through the wave's own LDS (fp32 rows of over 256 bytes in two halves), then rows of 16-byte pieces
   __syncthreads();
   if (!live) return;
-  constexpr int ES = (int)sizeof(T), HALVES = ES / 2, COLS = 128 / HALVES, ROWB = COLS * ES;   // 256 bytes a row
-  unsigned char* mine = sm + wave * 64 * ROWB;
+  constexpr int ES = (int)sizeof(T), HALVES = 32 * NT_ * ES > 256 ? 2 : 1, COLS = 32 * NT_ / HALVES, ROWB = COLS * ES;
+  constexpr int PP = ROWB / 16, RP = 64 / PP;              // pieces of a row, rows of an instruction
+  static_assert(WAVES * 32 * MT_ * ROWB <= STAGES * STAGE, "the outputs fit the stages' LDS");
+  unsigned char* mine = sm + wave * 32 * MT_ * ROWB;
   const bool wide = p.ldc % (16 / ES) == 0 && ((uintptr_t)p.c & 15) == 0;
 #pragma unroll
   for (int hh = 0; hh < HALVES; ++hh) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < MT_; ++j) {
       const int row = 32 * j + r31;
       const long m = m0 + wm + row;
       const float as = m < p.m ? p.as[m] : 0.f;
 #pragma unroll
-      for (int i = hh * 4 / HALVES; i < (hh + 1) * 4 / HALVES; ++i) {
+      for (int i = hh * NT_ / HALVES; i < (hh + 1) * NT_ / HALVES; ++i) {
         float v[16];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
@@ -264,7 +272,7 @@ __global__ void __launch_bounds__(NT, 2) k_linear_fp8(const LinArgs p, int tiles
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const int at = (32 * i + 8 * g + 4 * half - hh * COLS) * ES;
-          unsigned char* to = mine + row * ROWB + ((at & ~15) ^ ((row & 15) << 4)) + (at & 15);
+          unsigned char* to = mine + row * ROWB + ((at & ~15) ^ ((row & (PP - 1)) << 4)) + (at & 15);
           if constexpr (ES == 2) *(uint2*)to = make_uint2(pack_bf16x2(v[4 * g], v[4 * g + 1]), pack_bf16x2(v[4 * g + 2], v[4 * g + 3]));
           else *(float4*)to = make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
         }
@@ -272,9 +280,9 @@ __global__ void __launch_bounds__(NT, 2) k_linear_fp8(const LinArgs p, int tiles
     }
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int t = 0; t < 16; ++t) {                        // 4 rows of 16 pieces an instruction
-      const int row = t * 4 + (lane >> 4), piece = lane & 15;
-      const u32x4 v = *(const u32x4*)(mine + row * ROWB + ((piece ^ (row & 15)) << 4));
+    for (int t = 0; t < 32 * MT_ / RP; ++t) {
+      const int row = t * RP + lane / PP, piece = lane % PP;
+      const u32x4 v = *(const u32x4*)(mine + row * ROWB + ((piece ^ (row & (PP - 1))) << 4));
       const long m = m0 + wm + row;
       const int n = n0 + wn + hh * COLS + piece * (16 / ES);
       if (m >= p.m || n >= p.n) continue;
@@ -291,22 +299,36 @@ __global__ void __launch_bounds__(NT, 2) k_linear_fp8(const LinArgs p, int tiles
   }
 }
 
-// Up to this many rows take the few-rows form: its blocks re-read w once per 64 rows
-constexpr long FEW = 64;
-
-template <typename T> int launch(const LinArgs& p, hipStream_t s) {
-  if (p.m <= FEW) {
-    const unsigned g = hv_cdiv(p.n, 16);
-    if (p.m <= 16) k_linear_fp8_rows<T, 1><<<g, 512, 0, s>>>(p);
-    else if (p.m <= 32) k_linear_fp8_rows<T, 2><<<g, 512, 0, s>>>(p);
-    else k_linear_fp8_rows<T, 4><<<g, 512, 0, s>>>(p);
-  } else {
-    const long tm = hv_cdiv(p.m, BM), tn = hv_cdiv(p.n, BN);
-    if (tm * tn > (1L << 22)) return HV_EUNSUPPORTED;     // a grid stays below 2^32 threads
-    k_linear_fp8<T><<<(unsigned)(tm * tn), NT, 0, s>>>(p, (int)tm, (int)tn);
-  }
+template <typename T, int WN, int WM, int NT_, int MT_, int STAGES> int launch_tiles(const LinArgs& p, hipStream_t s) {
+  const long tm = hv_cdiv(p.m, 32 * MT_ * WM), tn = hv_cdiv(p.n, 32 * NT_ * WN);
+  if (tm * tn > (1L << 22)) return HV_EUNSUPPORTED;       // a grid stays below 2^32 threads
+  k_linear_fp8<T, WN, WM, NT_, MT_, STAGES><<<(unsigned)(tm * tn), 64 * WN * WM, 0, s>>>(p, (int)tm, (int)tn);
   HV_CHECK_LAUNCH();
   return HV_OK;
+}
+
+template <typename T> int launch_rows(const LinArgs& p, hipStream_t s) {
+  const dim3 g(hv_cdiv(p.n, 16), p.m <= 64 ? 1 : hv_cdiv(p.m, 64));
+  if (g.y > 65535) return HV_EUNSUPPORTED;
+  if (p.m <= 16) k_linear_fp8_rows<T, 1><<<g, 512, 0, s>>>(p);
+  else if (p.m <= 32) k_linear_fp8_rows<T, 2><<<g, 512, 0, s>>>(p);
+  else k_linear_fp8_rows<T, 4><<<g, 512, 0, s>>>(p);
+  HV_CHECK_LAUNCH();
+  return HV_OK;
+}
+
+// The form with the least estimated time: rounds of 256 blocks (one a CU) times what a round takes per 128 codes of k.
+// Measured, us per 128 codes: few-rows form 0.13 / 0.2 / 0.3 (16 / 32 / 64 rows a block), tiles of 64 / 128 / 256: 0.43 /
+// 0.93 / 1.4 (k = 8192, 4096 outputs: 64 rows 22.0 / 29.5 / 60.3 / 61.5 us, 256 rows 81.1 / 30.5 / 61.0 / 91.1, 1024 rows
+// 315 / 110 / 64.4 / 92.3, 4096 rows 1249 / 427 / 238 / 118; k = 1024, 8192 outputs: 128 rows 16.9 / 6.8 / 11.9 / 13.8).
+template <typename T> int launch(const LinArgs& p, hipStream_t s) {
+  auto rounds = [&](long blocks) { return (double)((blocks + 255) / 256); };
+  auto tiles = [&](int b) { return rounds((long)hv_cdiv(p.m, b) * hv_cdiv(p.n, b)); };
+  const double few = rounds((long)hv_cdiv(p.n, 16) * hv_cdiv(p.m, 64)) * (p.m <= 16 ? 0.13 : p.m <= 32 ? 0.2 : 0.3);
+  const double t64 = tiles(64) * 0.43, t128 = tiles(128) * 0.93, t256 = tiles(256) * 1.4;
+  if (few <= t64 && few <= t128 && few <= t256) return launch_rows<T>(p, s);
+  if (t64 <= t128 && t64 <= t256) return launch_tiles<T, 2, 2, 1, 1, 6>(p, s);
+  return t128 <= t256 ? launch_tiles<T, 2, 2, 2, 2, 3>(p, s) : launch_tiles<T, 2, 4, 4, 2, 2>(p, s);
 }
 
 }  // namespace

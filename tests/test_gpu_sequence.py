@@ -278,6 +278,43 @@ def test_packed_attention_long_history(gpu_device):
             check(lse, val["lse"], tol["lse"], "lse")
 
 
+FEW_ROWS = {"ragged": ([1, 0, 3, 40, 2], [5000, 700, 0, 3001, 12]), "one": ([9], [1537]), "blind": ([50, 1], [20, 5000]),
+            "two tiles": ([33], [2049]), "many": ([1] * 70, [1040 + 7 * i for i in range(70)])}
+
+
+@pytest.mark.parametrize("name", list(FEW_ROWS))
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype,hq,hkv,d", [(BF, 4, 2, 128), (BF, 2, 2, 40), (F32, 3, 1, 64), (F32, 2, 2, 128)])
+def test_packed_attention_few_rows(gpu_device, name, causal, dtype, hq, hkv, d):
+    """Averages of a few rows and over 512 keys a sequence and 32 rows: the form that splits the keys, and its gradients."""
+    from hv_amd import ops, train_fn
+    lq, lk = FEW_ROWS[name]
+    q, k, v, do, cq, ck = packed_inputs(lq, lk, hq, hkv, d, dtype, 21, before=2, spare=3)
+    out, lse = ops.attention_packed(q, k, v, cq, ck, causal=causal, return_lse=True)
+    val, tol = reference(q, k, v, cq, ck, causal, d ** -0.5, do)
+    check(out, val["out"], tol["out"], "out")
+    check(lse, val["lse"], tol["lse"], "lse")
+    for t in (q, k, v):
+        t.requires_grad_(True)
+    trained = train_fn.attention_packed(q, k, v, cq, ck, causal=causal)
+    assert torch.equal(trained, out)
+    for n, t in zip(("dq", "dk", "dv"), torch.autograd.grad(trained, (q, k, v), do)):
+        check(t, val[n], tol[n], n)
+
+
+def test_packed_attention_more_shapes_of_blocks(gpu_device):
+    """Enough rows for one wave per 32 rows (no shared keys), and row parts of the key tiles in the backward."""
+    from hv_amd import train_fn
+    for lq, hq, hkv, d, dtype in (([2100, 1300, 700], 16, 16, 32, BF), ([1500], 12, 4, 64, BF), ([900, 1], 4, 1, 128, F32)):
+        q, k, v, do, cq, ck = packed_inputs(lq, lq, hq, hkv, d, dtype, 22)
+        for t in (q, k, v):
+            t.requires_grad_(True)
+        out = train_fn.attention_packed(q, k, v, cq, ck, causal=True)
+        val, tol = reference(q, k, v, cq, ck, True, d ** -0.5, do)
+        for n, t in zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, (q, k, v), do))):
+            check(t, val[n], tol[n], n)
+
+
 def test_packed_attention_offsets_past_32_bits(gpu_device):
     """A history whose rows lie more than 2^32 bytes apart."""
     from hv_amd import ops
@@ -490,7 +527,7 @@ def test_quantize_rows(gpu_device, rows, cols, dtype):
 ACTS = {"none": lambda x: x, "relu": lambda x: x.clamp_min(0), "silu": lambda x: x * torch.sigmoid(x),
         "gelu": lambda x: 0.5 * x * torch.erfc(-x / 2 ** 0.5), "leaky": lambda x: torch.where(x > 0, x, 0.1 * x),
         "sigmoid": torch.sigmoid}
-LINEAR = [(1, 1, 16), (1, 4096, 256), (2, 33, 48), (4, 130, 1024), (7, 257, 2064), (16, 64, 128), (17, 100, 320), (33, 31, 64),
+LINEAR = [(200, 1000, 512), (130, 8200, 160), (1100, 2100, 208), (600, 4200, 128), (2100, 8200, 64), (1, 1, 16), (1, 4096, 256), (2, 33, 48), (4, 130, 1024), (7, 257, 2064), (16, 64, 128), (17, 100, 320), (33, 31, 64),
           (64, 1000, 4096), (129, 128, 128), (128, 255, 272), (300, 520, 96), (257, 129, 2048), (1000, 768, 256)]
 
 
