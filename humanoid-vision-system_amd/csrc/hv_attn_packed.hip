@@ -1117,21 +1117,26 @@ constexpr long MAX_BLOCKS = 1L << 24;                    // a grid stays below 2
 // blocks that cover `total` rows in nseq sequences and the two ranges outside of them, BM packed rows each
 long tile_bound(long total, int nseq, int G, int BM) { return total * G / BM + nseq + 2; }
 
+// rows of the parts' workspace
+size_t part_rows(const hv_attn_packed_args& a, long n) { return (size_t)((a.total_k + n - 1) / n) * a.total_q * a.hq; }
+
 // Keys of a part in the few-rows form, 0: the tile form.  The few-rows form reads a sequence's keys once per 32 of its rows
 // and needs a second launch; the tile form gives one block all the keys of 64 or 128 rows, 128 keys a step.  Averages per
 // sequence decide: few rows where there are 512 keys for it and for each 32 rows (at most 8 times).  Measured, tile / few
 // rows, us: 1 x 4 rows, 4096 keys of 128: 69 / 14; 8 x 4, 1024: 22 / 15; 64 x 4, 1024: 47 / 45; 8 x 64, 1024: 21 / 26; 1 x 64,
 // 4096: 59 / 22; 64 columns: 64 x 1, 512: 12 / 18; 8 x 64, 1024: 13 / 19; 1 x 128, 4096: 35 / 25.
-// Parts are sized for about four blocks per CU, 128 keys (one slab per wave) at least.
+// Parts are sized for about two blocks per CU (12 queries against 85 056 keys, 8 heads: 78 us, four 85 us), 128 keys (one slab per wave) at least.
 int part_keys(const hv_attn_packed_args& a) {
   if (a.nseq == 0 || a.total_q == 0 || a.total_k == 0) return 0;
   const long tiles = (a.total_q * (a.hq / a.hkv) + 32L * a.nseq - 1) / (32L * a.nseq);      // of 32 rows a sequence
   if (tiles > 8 || a.total_k < 512 * (tiles + 1) * a.nseq) return 0;
-  long n = (a.total_k * a.hkv + 1023) / 1024;
+  long n = (a.total_k * a.hkv + 511) / 512;
   n = (n + 127) / 128 * 128;
+  // longer parts where the workspace (the number of parts that one sequence with all the keys would have, for every row)
+  // would pass 256 MiB: many sequences, which are short against all keys together
+  while (n < a.total_k && part_rows(a, n) * (a.d + 4) * sizeof(float) > (256u << 20)) n *= 2;
   return (int)(n < 128 ? 128 : n);
 }
-size_t part_rows(const hv_attn_packed_args& a, int n) { return (size_t)((a.total_k + n - 1) / n) * a.total_q * a.hq; }
 
 template <typename T, int DP> void launch_keys(const Args& a, int n, hipStream_t s) {
   const size_t rows = part_rows(a, n);

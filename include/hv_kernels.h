@@ -751,10 +751,11 @@ int hv_stability_stats(int dtype, const void* x_in, const void* x_out, int rows,
  * of the same sequence, with causal != 0 only j <= i + (keys - queries of the sequence).  A query
  * row that sees no key, and every row of no sequence, gets 0 (lse -inf).  Query head h reads key /
  * value head h / (hq / hkv).  Offsets are read on the device and clamped to the tensors.
- * Rows may lie apart (*_row, *_head: strides in elements, the last dimension is dense); every row
- * start must be 16-byte aligned.  out, out_low, dq, dk, dv are dense [rows, heads, d]. */
+ * Rows may lie apart (*_row, *_head: strides in elements, 0 or more; the last dimension is dense); every
+ * row start must be 16-byte aligned.  Inside a sequence the values are finite (a hidden key is multiplied
+ * by 0); what other rows hold does not matter.  out, out_low, dq, dk, dv are dense [rows, heads, d]. */
 typedef struct hv_attn_packed_args {
-  int dtype, hq, hkv, d;        /* HV_F32 / HV_BF16; hq % hkv == 0; d % 8 == 0, d <= 128 */
+  int dtype, hq, hkv, d;        /* HV_F32 / HV_BF16; hq % hkv == 0, hq / hkv <= 64, hq <= 1024; d % 8 == 0, d <= 128 */
   int nseq, causal;
   float scale;                  /* > 0 */
   int pad_;
@@ -774,8 +775,9 @@ typedef struct hv_attn_packed_args {
 size_t hv_attn_packed_args_bytes(void);   /* sizeof, for bindings */
 size_t hv_attn_packed_work_bytes(const hv_attn_packed_args* a);
 int hv_attn_packed(const hv_attn_packed_args* a, hv_stream_t stream);
-/* dq, dk, dv from q, k, v, out (+ out_low), lse and dout; gradients of a shared key / value head are
-   summed over its query heads in fp32; rows of no sequence get 0.  No atomics. */
+/* dq (NULL: not wanted), dk and dv (both or neither) from q, k, v, out (+ out_low), lse and dout; gradients of a
+   shared key / value head are summed over its query heads in fp32; rows of no sequence get 0.  No atomics: equal
+   calls give equal bits.  64 rows of q and dout lie within 2^29 elements. */
 size_t hv_attn_packed_backward_work_bytes(const hv_attn_packed_args* a);
 int hv_attn_packed_backward(const hv_attn_packed_args* a, hv_stream_t stream);
 
@@ -800,7 +802,8 @@ int hv_add_rmsnorm_backward(int r_dtype, const void* sum, const float* rstd, con
 int hv_quantize_rows_fp8(int dtype, const void* x, long ld, long rows, int cols, void* codes, float* scale,
                          hv_stream_t stream);
 /* c[m, n] = act(a_scale[m] w_scale[n] sum_k a[m, k] w[n, k] + bias[n]): a, w e4m3 (nn.Linear, e.g. the MLP of
-   vit_encoder_decoder.py:146-152, on 8-bit rows); sums in fp32; c fp32 or bf16.  k, lda and ldw are multiples
+   vit_encoder_decoder.py:146-152, on 8-bit rows); sums in fp32 (the 8-bit matrix instruction itself cuts the products
+   of 8 consecutive k 13 binary places below their largest before it adds them); c fp32 or bf16.  k, lda and ldw are multiples
    of 16 and a, w 16-byte aligned.  work: hv_linear_fp8_work_bytes. */
 size_t hv_linear_fp8_work_bytes(long m, int n, int k);
 int hv_linear_fp8(const void* a, long lda, const float* a_scale, const void* w, long ldw, const float* w_scale,

@@ -641,6 +641,71 @@ def test_prenorm_block_on_packed_images(gpu_device):
     check(y, Y2, (unit(BF) + D * E) * Y2.abs() + 4 * E * rs2, "norm")
 
 
+def test_inference_block_in_a_graph(gpu_device):
+    """norm -> 8-bit layer -> attention of new tokens against a history (its workspace inside the graph) -> norm, captured
+    twice side by side and replayed between eager calls on other inputs: the bits of the eager calls."""
+    from hv_amd import ops
+    g = torch.Generator().manual_seed(16)
+    D, hq, hkv, d = 256, 8, 2, 32
+    lk = [3000, 1500, 40]
+    cq, ck = offsets([1, 1, 1]).to(gpu_device), offsets(lk).to(gpu_device)
+    w = (1 + 0.1 * torch.randn(D, generator=g)).to(gpu_device)
+    w8, ws = ops.quantize_rows_fp8((torch.randn(hq * d, D, generator=g) / 16).to(gpu_device))
+    k, v = (torch.randn(sum(lk), hkv, d, generator=g).to(BF).to(gpu_device) for _ in range(2))
+
+    def step(x, r):
+        h, hs, s = ops.add_rmsnorm_fp8(x, r, w)
+        o = ops.attention_packed(ops.linear_fp8(h, hs, w8, ws).view(3, hq, d), k, v, cq, ck, causal=True)
+        return (*ops.add_rmsnorm(o.view(3, D), s, w), o)
+
+    inputs = [(torch.randn(3, D, generator=g).to(BF).to(gpu_device), torch.randn(3, D, generator=g).to(gpu_device)) for _ in range(4)]
+    static = [tuple(t.clone() for t in inputs[0]) for _ in range(2)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*static[0])
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = [torch.cuda.CUDAGraph() for _ in static]
+    res = []
+    for gr, st in zip(graphs, static):
+        with torch.cuda.graph(gr):
+            res.append(step(*st))
+    for i in range(3):
+        for st, new in zip(static, (inputs[i], inputs[i + 1])):
+            for s, t in zip(st, new):
+                s.copy_(t)
+        for gr in graphs:
+            gr.replay()
+        eager = [step(*inputs[i]), step(*inputs[i + 1])]
+        torch.cuda.synchronize()
+        for a, b in zip(res, eager):
+            assert all(torch.equal(x, y) for x, y in zip(a, b)), i
+
+
+def test_add_rmsnorm_accumulates_into_leaves(gpu_device):
+    """x and residual of one type get one gradient tensor: their .grad stay apart, also over two passes."""
+    from hv_amd import train_fn
+    x, r, w = (torch.randn(5, 64, device=gpu_device).requires_grad_(True) for _ in range(3))
+    w = torch.ones(64, device=gpu_device).requires_grad_(True)
+    dy = torch.randn(5, 64, device=gpu_device)
+    for n in (1, 2):
+        y, s = train_fn.add_rmsnorm(x, r, w)
+        y.backward(dy)
+        assert x.grad.data_ptr() != r.grad.data_ptr() and torch.equal(x.grad, r.grad)
+        if n == 1:
+            first = x.grad.clone()
+    assert torch.equal(x.grad, 2 * first)
+    with torch.no_grad():
+        x.grad.zero_()
+    assert (r.grad != 0).any()
+    y, s = train_fn.add_rmsnorm(x, x, w)                           # one tensor in both places
+    (gx,) = torch.autograd.grad(y, x, dy)
+    z = x.detach().clone().requires_grad_(True)
+    y, s = train_fn.add_rmsnorm(z * 2, torch.zeros_like(z), w)
+    (gz,) = torch.autograd.grad(y, z, dy)
+    check(gx, gz.double().cpu(), 64 * E * (1 + gz.double().cpu().abs()), "x twice")
+
+
 def test_training_block_gradients(gpu_device):
     """norm -> packed attention -> norm in fp32, differentiated as a whole, against 64-bit autograd: every value passes
     fewer than 64 sums of at most 256 terms, so the gradients agree to 2e-5 of their norm (2^-24 * 256 = 1.5e-5)."""
