@@ -233,7 +233,10 @@ __device__ __forceinline__ void dma16(const void* src, unsigned lds) {
 #pragma clang diagnostic pop
 }
 // the same from base + off, base the same for the whole wave
-__device__ __forceinline__ void dma16_at(const void* base, unsigned off, unsigned lds) {
+__device__ __forceinline__ void dma16_at(const void* wave_base, unsigned off, unsigned lds) {
+  const uint64_t b = (uint64_t)wave_base;
+  const uint64_t base = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)b) |
+                        (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(b >> 32)) << 32;
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
   asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
@@ -907,18 +910,19 @@ __global__ void __launch_bounds__(NT, DP * sizeof(T) * KS > 256 ? 1 : 2) k_attn_
 
 // dK, dV: a block holds 64 keys and walks over the packed rows of its sequence (all heads of the group), 64 rows a tile:
 // waves 0 and 2 own the first 32 keys, 1 and 3 the others; 0 and 1 take a tile's first 32 rows, 2 and 3 the others, and
-// the two halves are added through LDS at the end.  (A block of 128 keys whose waves all walk over every row has the same
-// LDS traffic and half as many, twice as long blocks: 4096 + 2991 causal tokens, 4 heads, 760 against 700 us.)  Where the
-// keys give few blocks, `parts` blocks share a key tile's rows and write fp32 parts that k_attn_packed_sum adds in order.
+// the two halves are added through LDS at the end.  (Blocks of 128 keys whose waves all walk over every row: half as many,
+// twice as long.)  dK and dV of 32 keys fill 128 registers a lane, so K and V stay in LDS and Q and dO have one buffer each:
+// two blocks then share a CU and one computes while the other's tile arrives.  (4096 + 2991 causal tokens, 16 heads of 128 on
+// 4: K and V in registers, two buffers, one block a CU 386 us, this 314.)  Where the keys give few blocks, `parts` blocks share
+// a key tile's rows and write fp32 parts that k_attn_packed_sum adds in order.
 template <typename T, int DP>
-__global__ void __launch_bounds__(NT, DP * sizeof(T) >= 256 ? 1 : 2) k_attn_packed_dkv(const Args a, const float* __restrict__ delta,
+__global__ void __launch_bounds__(NT, DP * sizeof(T) > 256 ? 1 : 2) k_attn_packed_dkv(const Args a, const float* __restrict__ delta,
                                                                                           float* __restrict__ part_dk,
                                                                                           int parts) {
   using L = Lay<T, DP>;
-  auto fence = [] { if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0); };
   constexpr int BK = KEYS, BR = 64, TB = BR * L::ROWB;
-  __shared__ __align__(16) char smem[4 * TB];          // Q and dO, two buffers
-  __shared__ __align__(16) float st[2][2][BR];         // -lse log2 e and delta of the rows
+  __shared__ __align__(16) char smem[4 * TB];          // Q, dO, K, V
+  __shared__ __align__(16) float st[2][BR];           // -lse log2 e and delta of the rows         // -lse log2 e and delta of the rows
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
   const int part = blockIdx.x % parts, x = blockIdx.x / parts;          // a tile's parts side by side: long blocks first
   const int G = a.group.d, block = a.heads.div(x), kvh = a.heads.mod(x, block);
@@ -930,11 +934,6 @@ __global__ void __launch_bounds__(NT, DP * sizeof(T) >= 256 ? 1 : 2) k_attn_pack
   const int key = t.tile * BK + kh * 32 + (lane & 31);
   const bool real = key < t.len;
   const long krow = (long)t.start + key;
-  Frag<T> kf[L::NS], vf[L::NS];
-  load_row<T, DP>(kf, real ? (const T*)a.k + krow * a.k_row + (long)kvh * a.k_head : nullptr, a.d, h);
-  load_row<T, DP>(vf, real ? (const T*)a.v + krow * a.v_row + (long)kvh * a.v_head : nullptr, a.d, h);
-  settle(kf);
-  settle(vf);
   const int late = t.len - lq;
   // causal: row (token i) sees key j iff i >= j - late
   const int first_tok = a.causal ? max(t.tile * BK - late, 0) : 0;
@@ -947,6 +946,17 @@ __global__ void __launch_bounds__(NT, DP * sizeof(T) >= 256 ? 1 : 2) k_attn_pack
 #pragma unroll
   for (int i = 0; i < L::NDT; ++i) { dk[i] = zero16(); dv[i] = zero16(); }
   const View<T, DP> view(lane);
+  // K and V of the block, zeros behind the last key and column (there the tiles' rows hold copies)
+  for (int i = threadIdx.x; i < BK * L::CH; i += NT) {
+    const int row = i / L::CH, c = i % L::CH;
+    const bool in = t.tile * BK + row < t.len && c * L::EPC < a.d;
+    const long at = (long)t.start + t.tile * BK + row;
+    const int to = row * L::ROWB + ((c ^ L::f(row)) << 4);
+    *(u32x4*)(smem + 2 * TB + to) = in ? *(const u32x4*)((const T*)a.k + at * a.k_row + (long)kvh * a.k_head + c * L::EPC) : u32x4{0, 0, 0, 0};
+    *(u32x4*)(smem + 3 * TB + to) = in ? *(const u32x4*)((const T*)a.v + at * a.v_row + (long)kvh * a.v_head + c * L::EPC) : u32x4{0, 0, 0, 0};
+  }
+  const char* tk = smem + 2 * TB + kh * 32 * L::ROWB;    // this wave's keys
+  const char* tv = tk + TB;
   const T* qp = (const T*)a.q + (long)q0 * a.q_row + (long)kvh * G * a.q_head;
   const T* gp = (const T*)a.dout + (long)q0 * a.do_row + (long)kvh * G * a.do_head;
   const long sbase = (long)q0 * a.hq + (long)kvh * G;
@@ -968,46 +978,35 @@ __global__ void __launch_bounds__(NT, DP * sizeof(T) >= 256 ? 1 : 2) k_attn_pack
   };
   // from the last rows, which every block of the sequence needs, backwards: blocks that run together read the same tiles
   int tile = tn - 1 - part;
-  if (tile >= t0) {
-    sq.last(a.q_row, a.q_head, tile * used, rows, a.d, a.group, lds0);
-    sg.last(a.do_row, a.do_head, tile * used, rows, a.d, a.group, lds0 + TB);
-    stats(tile * used);
-  }
-  for (int buf = 0; tile >= t0; tile -= parts, buf ^= 1) {
+  for (bool first = true; tile >= t0; tile -= parts, first = false) {
     const int rr = tile * used;
+    __syncthreads();                                     // the tile before is no longer read
+    if (first) {
+      sq.last(a.q_row, a.q_head, rr, rows, a.d, a.group, lds0);
+      sg.last(a.do_row, a.do_head, rr, rows, a.d, a.group, lds0 + TB);
+    } else {
+      sq.send_tile((long)tile * toks * a.q_row, lds0);
+      sg.send_tile((long)tile * toks * a.do_row, lds0 + TB);
+    }
+    stats(rr);
     arrived();
-    if (threadIdx.x < BR) st[buf][0][threadIdx.x] = stat == NEG_INF ? 0.f : -stat * LOG2E;
-    else if (threadIdx.x < 2 * BR) st[buf][1][threadIdx.x - BR] = stat;
+    if (threadIdx.x < BR) st[0][threadIdx.x] = stat == NEG_INF ? 0.f : -stat * LOG2E;
+    else if (threadIdx.x < 2 * BR) st[1][threadIdx.x - BR] = stat;
     __syncthreads();
-    if (tile - parts >= t0) {
-      const unsigned at = lds0 + (buf ^ 1) * 2 * TB;
-      sq.send_tile((long)(tile - parts) * toks * a.q_row, at);
-      sg.send_tile((long)(tile - parts) * toks * a.do_row, at + TB);
-      stats((tile - parts) * used);
-    }
     const int j = rh * 32, rj = rr + j;
-    const char* tq = smem + buf * 2 * TB + j * L::ROWB;
+    const char* tq = smem + j * L::ROWB;
     const char* tg = tq + TB;
-    // All operands of a product are on their way before its first instruction, the second products' during the first ones:
-    // one wave per SIMD has nobody else to fill the LDS latency (each read just before its use: 472 us against the below).
     f32x16 s = zero16(), dp = zero16();
-    {
-      Frag<T> x[L::NS], y[L::NS];
 #pragma unroll
-      for (int i = 0; i < L::NS; ++i) { x[i] = view.rows(tq, i); y[i] = view.rows(tg, i); }
-      fence();
-#pragma unroll
-      for (int i = 0; i < L::NS; ++i) { s = mma16(x[i], kf[i], s); dp = mma16(y[i], vf[i], dp); }
+    for (int i = 0; i < L::NS; ++i) {
+      s = mma16(view.rows(tq, i), view.rows(tk, i), s);
+      dp = mma16(view.rows(tg, i), view.rows(tv, i), dp);
     }
-    Frag<T> x[L::NDT], y[L::NDT];
-#pragma unroll
-    for (int dt = 0; dt < L::NDT; ++dt) { x[dt] = view.cols(tg, dt); y[dt] = view.cols(tq, dt); }
-    fence();
     const int end = min(rr + used, rows);
     const bool edge = rj + 32 > end || a.group.div(rj) < wave_last;
 #pragma unroll
     for (int y = 0; y < 4; ++y) {
-      const f32x4 le = *(const f32x4*)&st[buf][0][j + 8 * y + 4 * h];
+      const f32x4 le = *(const f32x4*)&st[0][j + 8 * y + 4 * h];
 #pragma unroll
       for (int x = 0; x < 4; ++x) s[4 * y + x] = __builtin_amdgcn_exp2f(fmaf(s[4 * y + x], c2, le[x]));
     }
@@ -1020,21 +1019,18 @@ __global__ void __launch_bounds__(NT, DP * sizeof(T) >= 256 ? 1 : 2) k_attn_pack
     }
 #pragma unroll
     for (int y = 0; y < 4; ++y) {
-      const f32x4 dl = *(const f32x4*)&st[buf][1][j + 8 * y + 4 * h];
+      const f32x4 dl = *(const f32x4*)&st[1][j + 8 * y + 4 * h];
 #pragma unroll
       for (int x = 0; x < 4; ++x) dp[4 * y + x] = s[4 * y + x] * (dp[4 * y + x] - dl[x]);
     }
-    {
-      Frag<T> x1[L::NDT], y1[L::NDT];
-      const Frag<T> p = from_acc<T>(s, 0), ds = from_acc<T>(dp, 0);
 #pragma unroll
-      for (int dt = 0; dt < L::NDT; ++dt) { x1[dt] = view.cols(tg + 16 * L::ROWB, dt); y1[dt] = view.cols(tq + 16 * L::ROWB, dt); }
-      fence();
+    for (int i = 0; i < 2; ++i) {
+      const Frag<T> p = from_acc<T>(s, i), ds = from_acc<T>(dp, i);
 #pragma unroll
-      for (int dt = 0; dt < L::NDT; ++dt) { dv[dt] = mma16(x[dt], p, dv[dt]); dk[dt] = mma16(y[dt], ds, dk[dt]); }
-      const Frag<T> p1 = from_acc<T>(s, 1), ds1 = from_acc<T>(dp, 1);
-#pragma unroll
-      for (int dt = 0; dt < L::NDT; ++dt) { dv[dt] = mma16(x1[dt], p1, dv[dt]); dk[dt] = mma16(y1[dt], ds1, dk[dt]); }
+      for (int dt = 0; dt < L::NDT; ++dt) {
+        dv[dt] = mma16(view.cols(tg + 16 * i * L::ROWB, dt), p, dv[dt]);
+        dk[dt] = mma16(view.cols(tq + 16 * i * L::ROWB, dt), ds, dk[dt]);
+      }
     }
   }
   // the second half's sums, then the first half adds them
