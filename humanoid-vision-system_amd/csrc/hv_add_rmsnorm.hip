@@ -179,11 +179,11 @@ __global__ void __launch_bounds__(threads_of<TPR>()) k_add_rmsnorm(const NormArg
 }
 
 struct NormBackArgs {
-  const void* sum;
+  const void *x, *residual;       // the sum's operands, or the sum and null
   const float *rstd, *w;
   const void *dy, *dsum;
   long rows;
-  int cols, r_dtype, dy_dtype, dx_dtype;
+  int cols, x_dtype, r_dtype, dy_dtype, dx_dtype;
   void *dx, *dresidual;
   float* part;                    // [blocks, cols] column sums of dy s rstd
 };
@@ -217,8 +217,15 @@ __global__ void __launch_bounds__(threads_of<TPR>()) k_add_rmsnorm_back(const No
           to[i] = in(i) ? load_vec<VW>((const float*)from + base + (t + i * TPR) * VW) : Vec<VW>{};
       }
     };
-    read(n, a.sum, a.r_dtype);
+    read(n, a.x, a.x_dtype);
     read(g, a.dy, a.dy_dtype);
+    if (a.residual) {
+      read(d, a.residual, a.r_dtype);
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+#pragma unroll
+        for (int e = 0; e < VW; ++e) n[i].v[e] += d[i].v[e];
+    }
     if (a.dsum) {
       read(d, a.dsum, a.r_dtype);
     } else {
@@ -371,17 +378,21 @@ extern "C" size_t hv_add_rmsnorm_backward_work_floats(long rows, int cols) {
   return rows <= 0 || cols <= 0 ? 0 : (size_t)norm_blocks(rows, cols) * cols;
 }
 
-extern "C" int hv_add_rmsnorm_backward(int r_dtype, const void* sum, const float* rstd, const float* scale, int dy_dtype,
-                                       const void* dy, const void* dsum, long rows, int cols, int dx_dtype, void* dx,
-                                       void* dresidual, float* dscale, float* work, hv_stream_t stream) {
-  if (!is_float(r_dtype) || !is_float(dy_dtype) || (dx && !is_float(dx_dtype)) || rows < 0 || cols <= 0) return HV_EINVAL;
+extern "C" int hv_add_rmsnorm_backward(int x_dtype, const void* x, int r_dtype, const void* residual, const float* rstd,
+                                       const float* scale, int dy_dtype, const void* dy, const void* dsum, long rows, int cols,
+                                       int dx_dtype, void* dx, void* dresidual, float* dscale, float* work,
+                                       hv_stream_t stream) {
+  if (!is_float(x_dtype) || !is_float(r_dtype) || !is_float(dy_dtype) || (dx && !is_float(dx_dtype)) || rows < 0 || cols <= 0)
+    return HV_EINVAL;
   if (cols > MAX_COLS || rows > MAX_ROWS) return HV_EUNSUPPORTED;
-  if (!dscale || (rows > 0 && (!sum || !rstd || !scale || !dy || !work))) return HV_EINVAL;
+  if (!dscale || (rows > 0 && (!x || !rstd || !scale || !dy || !work))) return HV_EINVAL;
   hipStream_t s = (hipStream_t)stream;
   const int nb = rows > 0 ? norm_blocks(rows, cols) : 0;
   if (rows > 0) {
-    const bool wide = cols % 8 == 0 && a16(sum) && a16(scale) && a16(dy) && a16(dsum) && a16(dx) && a16(dresidual) && a16(work);
-    const NormBackArgs a{sum, rstd, scale, dy, dsum, rows, cols, r_dtype, dy_dtype, dx_dtype, dx, dresidual, work};
+    const bool wide = cols % 8 == 0 && a16(x) && a16(residual) && a16(scale) && a16(dy) && a16(dsum) && a16(dx) &&
+                      a16(dresidual) && a16(work);
+    const NormBackArgs a{x,    residual, rstd,    scale,    dy,       dsum, rows,
+                         cols, x_dtype,  r_dtype, dy_dtype, dx_dtype, dx,   dresidual, work};
 #define HV_NORM_CALL(VW, TPR, V) k_add_rmsnorm_back<VW, TPR, V><<<nb, threads_of<TPR>(), 0, s>>>(a)
     HV_ROW_SHAPE(cols, wide, HV_NORM_CALL);
 #undef HV_NORM_CALL

@@ -268,7 +268,7 @@ _SIGS = {
     "hv_attn_packed_backward": ([vp, vp], i32),
     "hv_add_rmsnorm": ([i32, vp, i32, vp, i64, i32, f32, vp, vp, i32, vp, vp, vp, vp], i32),
     "hv_add_rmsnorm_backward_work_floats": ([i64, i32], C.c_size_t),
-    "hv_add_rmsnorm_backward": ([i32, vp, vp, vp, i32, vp, vp, i64, i32, i32, vp, vp, vp, vp, vp], i32),
+    "hv_add_rmsnorm_backward": ([i32, vp, i32, vp, vp, vp, i32, vp, vp, i64, i32, i32, vp, vp, vp, vp, vp], i32),
     "hv_quantize_rows_fp8": ([i32, vp, i64, i64, i32, vp, vp, vp], i32),
     "hv_linear_fp8_work_bytes": ([i64, i32, i32], C.c_size_t),
     "hv_linear_fp8": ([vp, i64, vp, vp, i64, vp, vp, i32, i64, i32, i32, i32, vp, i64, vp, vp], i32),

@@ -542,28 +542,31 @@ def add_rmsnorm_train(x: Tensor, residual: Tensor, scale: Tensor, eps: float, ou
     return y, s, rstd
 
 
-def add_rmsnorm_backward(s: Tensor, rstd: Tensor, scale: Tensor, dy: Tensor, ds: Optional[Tensor],
-                         dx_dtype: Optional[torch.dtype], need_residual: bool = True):
-    """(dx, dresidual, dscale) of add_rmsnorm_train: dx and dresidual are one value in two dtypes -- the same
-    tensor where the dtypes agree; dx_dtype None / need_residual False: not wanted."""
-    _contig(s, "s")
-    _contig(dy, "dy")
-    if ds is not None and (ds.shape != s.shape or ds.dtype != s.dtype or not ds.is_contiguous()):
-        raise ValueError("add_rmsnorm_backward: ds is not like s")
-    if dy.shape != s.shape:
-        raise ValueError("add_rmsnorm_backward: dy and s disagree")
-    cols = s.shape[-1]
-    rows = s.numel() // cols
-    shared = dx_dtype == s.dtype
-    dx = torch.empty(s.shape, device=s.device, dtype=dx_dtype) if dx_dtype is not None else None
-    dr = torch.empty_like(s) if need_residual and not shared else None
-    dscale = torch.empty(cols, device=s.device, dtype=torch.float32)
+def add_rmsnorm_backward(x: Tensor, residual: Optional[Tensor], rstd: Tensor, scale: Tensor, dy: Tensor,
+                         ds: Optional[Tensor], dx_dtype: Optional[torch.dtype], r_dtype: torch.dtype,
+                         need_residual: bool = True):
+    """(dx, dresidual, dscale) of add_rmsnorm_train from the sum's operands x and residual, or from the stored fp32
+    sum as x with residual None.  dx and dresidual are one value in two dtypes -- the same tensor where the dtypes
+    agree; dx_dtype None / need_residual False: not wanted."""
+    for name, t in (("x", x), ("dy", dy), ("residual", residual), ("ds", ds)):
+        if t is not None:
+            _contig(t, name)
+            if t.shape != x.shape:
+                raise ValueError(f"add_rmsnorm_backward: {name} {tuple(t.shape)} is not like x {tuple(x.shape)}")
+    if (ds is not None and ds.dtype != r_dtype) or (residual is not None and residual.dtype != r_dtype):
+        raise TypeError("add_rmsnorm_backward: ds and the residual have one dtype")
+    cols = x.shape[-1]
+    rows = x.numel() // cols
+    shared = dx_dtype == r_dtype
+    dx = torch.empty(x.shape, device=x.device, dtype=dx_dtype) if dx_dtype is not None else None
+    dr = torch.empty(x.shape, device=x.device, dtype=r_dtype) if need_residual and not shared else None
+    dscale = torch.empty(cols, device=x.device, dtype=torch.float32)
     lib = L.lib()
-    work = _work(lib.hv_add_rmsnorm_backward_work_floats(rows, cols), s.device)
-    with on_device(s) as stream:
-        check(lib.hv_add_rmsnorm_backward(dtype_code(s.dtype), s.data_ptr(), rstd.data_ptr(), scale.data_ptr(),
-                                          dtype_code(dy.dtype), dy.data_ptr(), ptr(ds), rows, cols,
-                                          dtype_code(dx_dtype) if dx is not None else 0, ptr(dx), ptr(dr),
+    work = _work(lib.hv_add_rmsnorm_backward_work_floats(rows, cols), x.device)
+    with on_device(x) as stream:
+        check(lib.hv_add_rmsnorm_backward(dtype_code(x.dtype), x.data_ptr(), dtype_code(r_dtype), ptr(residual),
+                                          rstd.data_ptr(), scale.data_ptr(), dtype_code(dy.dtype), dy.data_ptr(), ptr(ds),
+                                          rows, cols, dtype_code(dx_dtype) if dx is not None else 0, ptr(dx), ptr(dr),
                                           dscale.data_ptr(), work.data_ptr(), stream), "hv_add_rmsnorm_backward")
     return dx, (dx if shared and need_residual else dr), dscale
 

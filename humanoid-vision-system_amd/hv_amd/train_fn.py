@@ -478,6 +478,8 @@ class AttentionFn(torch.autograd.Function):
 class PackedAttentionFn(torch.autograd.Function):
     """Attention over packed sequences (ops.attention_packed) with its gradient."""
 
+    _hv_carries_state = True                             # reads no model options
+
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k, causal: bool, scale):
         out, low, lse, ctx.call = T.attention_packed_train(q, k, v, cu_q, cu_k, causal, scale)
@@ -502,29 +504,35 @@ def attention_packed(q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Option
 
 
 class AddRMSNormFn(torch.autograd.Function):
-    """Residual addition + RMS norm (ops.add_rmsnorm) with its gradient: returns (y, s)."""
+    """Residual addition + RMS norm (ops.add_rmsnorm) with its gradient: returns (y, s).  An fp32 sum is kept for the
+    backward; a bf16 one is formed again from its operands (its rounding would be the weight gradient's)."""
+
+    _hv_carries_state = True                             # reads no model options
 
     @staticmethod
     def forward(ctx, x, residual, scale, eps: float, out_dtype):
         w = f32(scale)
         y, s, rstd = T.add_rmsnorm_train(x, residual, w, eps, out_dtype)
         ctx.set_materialize_grads(False)
-        ctx.dtypes = (x.dtype, scale.dtype)
-        ctx.save_for_backward(s, rstd, w)
+        ctx.dtypes = (x.dtype, residual.dtype, scale.dtype)
+        if residual.dtype == torch.float32:
+            ctx.save_for_backward(s, None, rstd, w)
+        else:
+            ctx.save_for_backward(x, residual, rstd, w)
         return y, s
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, ds):
-        s, rstd, w = ctx.saved_tensors
-        x_dtype, w_dtype = ctx.dtypes
+        x, residual, rstd, w = ctx.saved_tensors
+        x_dtype, r_dtype, w_dtype = ctx.dtypes
         if dy is None:                                   # only the sum was used
             if ds is None:
                 return None, None, None, None, None
             return ds.to(x_dtype), ds, None, None, None
         ds = None if ds is None else ds.contiguous()
-        dx, dr, dw = T.add_rmsnorm_backward(s, rstd, w, dy.contiguous(), ds, x_dtype if _need(ctx, 0) else None,
-                                            _need(ctx, 1))
+        dx, dr, dw = T.add_rmsnorm_backward(x, residual, rstd, w, dy.contiguous(), ds, x_dtype if _need(ctx, 0) else None,
+                                            r_dtype, _need(ctx, 1))
         return dx, dr, dw.to(w_dtype), None, None
 
 

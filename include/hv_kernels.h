@@ -791,12 +791,14 @@ enum { HV_E4M3 = 3 /* OCP 8-bit float, 4 exponent and 3 mantissa bits */ };
 int hv_add_rmsnorm(int x_dtype, const void* x, int r_dtype, const void* residual, long rows, int cols, float eps,
                    const float* scale, void* sum, int y_dtype, void* y, float* y_scale, float* rstd,
                    hv_stream_t stream);
-/* dx (dx_dtype) and dresidual (r_dtype), the same values (either may be NULL), and dscale [cols] fp32 from the
-   stored sum, rstd, dy (dy_dtype) and dsum (r_dtype; NULL: the sum has no consumer).  No atomics. */
+/* dx (dx_dtype) and dresidual (r_dtype), the same values (either may be NULL), and dscale [cols] fp32 from rstd, dy
+   (dy_dtype), dsum (r_dtype; NULL: the sum has no consumer) and the sum itself: x + residual, or x alone where residual is
+   NULL -- an fp32 sum as the forward stored it; a bf16 sum is formed again from its operands, its rounding would be
+   that of dscale.  No atomics. */
 size_t hv_add_rmsnorm_backward_work_floats(long rows, int cols);
-int hv_add_rmsnorm_backward(int r_dtype, const void* sum, const float* rstd, const float* scale, int dy_dtype,
-                            const void* dy, const void* dsum, long rows, int cols, int dx_dtype, void* dx,
-                            void* dresidual, float* dscale, float* work, hv_stream_t stream);
+int hv_add_rmsnorm_backward(int x_dtype, const void* x, int r_dtype, const void* residual, const float* rstd,
+                            const float* scale, int dy_dtype, const void* dy, const void* dsum, long rows, int cols,
+                            int dx_dtype, void* dx, void* dresidual, float* dscale, float* work, hv_stream_t stream);
 
 /* rows of x (leading dimension ld) -> e4m3 codes, dense [rows, cols], and the scale of each row as above */
 int hv_quantize_rows_fp8(int dtype, const void* x, long ld, long rows, int cols, void* codes, float* scale,

@@ -450,6 +450,23 @@ def test_add_rmsnorm_gradients(gpu_device, rows, cols, xd, rd):
             check(dw, (DY * n).sum(0), (ur + row + (rows + 8) * E) * mag, "dscale")
 
 
+def test_add_rmsnorm_weight_gradient_of_a_bf16_stream(gpu_device):
+    """The weight's gradient does not carry the stored sum's rounding: rows of dy n are summed in fp32 from the unrounded
+    sum, so it is off by (cols / 2 + rows + 24) e of sum|dy n|."""
+    from hv_amd import train_fn
+    g = torch.Generator().manual_seed(31)
+    for rows, cols, xd in ((7, 104, BF), (600, 1024, BF), (40, 77, F32)):
+        x = torch.randn(rows, cols, generator=g).to(xd).to(gpu_device)
+        r = torch.randn(rows, cols, generator=g).to(BF).to(gpu_device)
+        w = (1 + 0.3 * torch.randn(cols, generator=g)).to(gpu_device).requires_grad_(True)
+        dy = torch.randn(rows, cols, generator=g).to(xd).to(gpu_device)
+        y, s = train_fn.add_rmsnorm(x, r, w, 1e-6)
+        (dw,) = torch.autograd.grad(y, w, dy)
+        S, rs, _ = norm_reference(x, r, w.detach(), 1e-6)
+        n = S * rs * dy.double().cpu()
+        check(dw, n.sum(0), (cols / 2 + rows + 24) * E * n.abs().sum(0), "dscale")
+
+
 def test_add_rmsnorm_edges(gpu_device):
     """Zero rows, an infinity, NaN, no residual, no rows, misaligned rows, more than two dimensions."""
     from hv_amd import ops

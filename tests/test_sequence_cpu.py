@@ -111,7 +111,8 @@ def test_c_entries_refuse():
                 (0, p, 0, p, 2, 32, 1e-8, p, p, 2, p, None, None)):
         assert lib.hv_add_rmsnorm(*bad, None) == -1, bad
     assert lib.hv_add_rmsnorm(0, p, 0, p, 2, 32769, 1e-8, p, p, 0, p, None, None, None) == -2
-    assert lib.hv_add_rmsnorm_backward(0, p, p, p, 0, None, p, 2, 32, 0, p, p, p, p, None) == -1
+    assert lib.hv_add_rmsnorm_backward(0, p, 0, p, p, p, 0, None, p, 2, 32, 0, p, p, p, p, None) == -1
+    assert lib.hv_add_rmsnorm_backward(0, p, 2, p, p, p, 0, p, p, 2, 32, 0, p, p, p, p, None) == -1
     assert lib.hv_quantize_rows_fp8(0, p, 16, 2, 32, p, p, None) == -1
     for bad, rc in (((p, 32, p, p, 32, p, None, 9, 4, 4, 32, 1, p, 4, None), -1), ((p, 32, p, p, 32, p, None, 0, 4, 4, 32, 2, p, 4, None), -1),
                     ((p, 16, p, p, 32, p, None, 0, 4, 4, 32, 1, p, 4, None), -1), ((p, 32, p, p, 32, p, None, 0, 4, 4, 24, 1, p, 4, None), -2),
