@@ -581,8 +581,8 @@ __global__ void __launch_bounds__(NT, DP * sizeof(T) * KS > 256 ? 1 : 2) k_attn_
 // wave's own LDS, both a slab ahead, so a wave has 2 * 32 rows in flight and a CU eight such waves.  Bytes bound it.
 // Partial sums (fp32, with their maxima) go to the workspace and are joined by k_attn_packed_join in a fixed order.
 template <typename T, int DP>
-__global__ void __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2) k_attn_packed_keys(const Args a, int part_keys, float* __restrict__ po,
-                                                         float4* __restrict__ pml) {
+__global__ void __launch_bounds__(NT, sizeof(T) == 4 && DP == 128 ? 1 : 2)
+k_attn_packed_keys(const Args a, int part_keys, float* __restrict__ po, float4* __restrict__ pml) {
   using L = Lay<T, DP>;
   constexpr int SB = 32 * L::ROWB;                       // a wave's V slab
   constexpr int JB = 32 * DP * 4;                        // a wave's O at the end, fp32
@@ -803,7 +803,8 @@ __global__ void __launch_bounds__(NT) k_attn_packed_delta(const Args a, float* _
 
 // dQ: the forward's walk over the keys with dO beside Q; dQ^T += K^T dS^T.  KS: as in the forward
 template <typename T, int DP, int KS>
-__global__ void __launch_bounds__(NT, DP * sizeof(T) * KS > 256 ? 1 : 2) k_attn_packed_dq(const Args a, const float* __restrict__ delta) {
+__global__ void __launch_bounds__(NT, DP * sizeof(T) * KS > 256 ? 1 : 2)
+k_attn_packed_dq(const Args a, const float* __restrict__ delta) {
   using L = Lay<T, DP>;
   constexpr int BM = 128 / KS, BN = L::ROWB > 256 ? 32 : 64, BT = BN * KS, TB = BT * L::ROWB;
   __shared__ __align__(16) char smem[4 * TB];          // K and V, two buffers
@@ -913,16 +914,15 @@ __global__ void __launch_bounds__(NT, DP * sizeof(T) * KS > 256 ? 1 : 2) k_attn_
 // the two halves are added through LDS at the end.  (Blocks of 128 keys whose waves all walk over every row: half as many,
 // twice as long.)  dK and dV of 32 keys fill 128 registers a lane, so K and V stay in LDS and Q and dO have one buffer each:
 // two blocks then share a CU and one computes while the other's tile arrives.  (4096 + 2991 causal tokens, 16 heads of 128 on
-// 4: K and V in registers, two buffers, one block a CU 386 us, this 314.)  Where the keys give few blocks, `parts` blocks share
+// 4: K and V in registers, two buffers, one block a CU 386 us, this 318.)  Where the keys give few blocks, `parts` blocks share
 // a key tile's rows and write fp32 parts that k_attn_packed_sum adds in order.
 template <typename T, int DP>
-__global__ void __launch_bounds__(NT, DP * sizeof(T) > 256 ? 1 : 2) k_attn_packed_dkv(const Args a, const float* __restrict__ delta,
-                                                                                          float* __restrict__ part_dk,
-                                                                                          int parts) {
+__global__ void __launch_bounds__(NT, DP * sizeof(T) > 256 ? 1 : 2)
+k_attn_packed_dkv(const Args a, const float* __restrict__ delta, float* __restrict__ part_dk, int parts) {
   using L = Lay<T, DP>;
   constexpr int BK = KEYS, BR = 64, TB = BR * L::ROWB;
   __shared__ __align__(16) char smem[4 * TB];          // Q, dO, K, V
-  __shared__ __align__(16) float st[2][BR];           // -lse log2 e and delta of the rows         // -lse log2 e and delta of the rows
+  __shared__ __align__(16) float st[2][BR];           // -lse log2 e and delta of the rows
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
   const int part = blockIdx.x % parts, x = blockIdx.x / parts;          // a tile's parts side by side: long blocks first
   const int G = a.group.d, block = a.heads.div(x), kvh = a.heads.mod(x, block);
@@ -952,8 +952,10 @@ __global__ void __launch_bounds__(NT, DP * sizeof(T) > 256 ? 1 : 2) k_attn_packe
     const bool in = t.tile * BK + row < t.len && c * L::EPC < a.d;
     const long at = (long)t.start + t.tile * BK + row;
     const int to = row * L::ROWB + ((c ^ L::f(row)) << 4);
-    *(u32x4*)(smem + 2 * TB + to) = in ? *(const u32x4*)((const T*)a.k + at * a.k_row + (long)kvh * a.k_head + c * L::EPC) : u32x4{0, 0, 0, 0};
-    *(u32x4*)(smem + 3 * TB + to) = in ? *(const u32x4*)((const T*)a.v + at * a.v_row + (long)kvh * a.v_head + c * L::EPC) : u32x4{0, 0, 0, 0};
+    const T* kp = (const T*)a.k + at * a.k_row + (long)kvh * a.k_head + c * L::EPC;
+    const T* vp = (const T*)a.v + at * a.v_row + (long)kvh * a.v_head + c * L::EPC;
+    *(u32x4*)(smem + 2 * TB + to) = in ? *(const u32x4*)kp : u32x4{0, 0, 0, 0};
+    *(u32x4*)(smem + 3 * TB + to) = in ? *(const u32x4*)vp : u32x4{0, 0, 0, 0};
   }
   const char* tk = smem + 2 * TB + kh * 32 * L::ROWB;    // this wave's keys
   const char* tv = tk + TB;
@@ -1121,17 +1123,18 @@ size_t part_rows(const hv_attn_packed_args& a, long n) { return (size_t)((a.tota
 // sequence decide: few rows where there are 512 keys for it and for each 32 rows (at most 8 times).  Measured, tile / few
 // rows, us: 1 x 4 rows, 4096 keys of 128: 69 / 14; 8 x 4, 1024: 22 / 15; 64 x 4, 1024: 47 / 45; 8 x 64, 1024: 21 / 26; 1 x 64,
 // 4096: 59 / 22; 64 columns: 64 x 1, 512: 12 / 18; 8 x 64, 1024: 13 / 19; 1 x 128, 4096: 35 / 25.
-// Parts are sized for about two blocks per CU (12 queries against 85 056 keys, 8 heads: 78 us, four 85 us), 128 keys (one slab per wave) at least.
+// Parts are sized for about two blocks per CU (12 queries against 85 056 keys, 8 heads: 78 us, four 85 us), 128 keys (one
+// slab per wave) at least.
 int part_keys(const hv_attn_packed_args& a) {
   if (a.nseq == 0 || a.total_q == 0 || a.total_k == 0) return 0;
   const long tiles = (a.total_q * (a.hq / a.hkv) + 32L * a.nseq - 1) / (32L * a.nseq);      // of 32 rows a sequence
   if (tiles > 8 || a.total_k < 512 * (tiles + 1) * a.nseq) return 0;
-  long n = (a.total_k * a.hkv + 511) / 512;
-  n = (n + 127) / 128 * 128;
+  const long n0 = min((a.total_k * a.hkv + 511) / 512, a.total_k);      // <= 2^30, also with more than 512 heads
+  long n = (n0 + 127) / 128 * 128;
   // longer parts where the workspace (the number of parts that one sequence with all the keys would have, for every row)
   // would pass 256 MiB: many sequences, which are short against all keys together
   while (n < a.total_k && part_rows(a, n) * (a.d + 4) * sizeof(float) > (256u << 20)) n *= 2;
-  return (int)(n < 128 ? 128 : n);
+  return (int)n;
 }
 
 template <typename T, int DP> void launch_keys(const Args& a, int n, hipStream_t s) {

@@ -88,7 +88,8 @@ __global__ void __launch_bounds__(512) k_linear_fp8_rows(const LinArgs p) {
       for (int d = 0; d < DEPTH; ++d)
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-          const i32x8 x = live[i] ? pair(*(const u32x4*)(pa[i] + k0 + d * step), *(const u32x4*)(pa[i] + k0 + d * step + 16)) : pair(none, none);
+          const i32x8 x = live[i] ? pair(*(const u32x4*)(pa[i] + k0 + d * step), *(const u32x4*)(pa[i] + k0 + d * step + 16))
+                                  : pair(none, none);
           acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[d], x, acc[i], 0, 0, 0, UNIT, 0, UNIT);
         }
     } else {

@@ -118,6 +118,10 @@ def test_c_entries_refuse():
                     ((p, 16, p, p, 32, p, None, 0, 4, 4, 32, 1, p, 4, None), -1), ((p, 32, p, p, 32, p, None, 0, 4, 4, 24, 1, p, 4, None), -2),
                     ((p + 1, 32, p, p, 32, p, None, 0, 4, 4, 32, 1, p, 4, None), -1), ((p, 32, None, p, 32, p, None, 0, 4, 4, 32, 1, p, 4, None), -1)):
         assert lib.hv_linear_fp8(*bad, None) == rc, bad
+    # more outputs than a grid has blocks for
+    assert lib.hv_linear_fp8(p, 16, p, p, 16, p, None, 0, 1 << 30, 1 << 28, 16, 1, p, 1 << 28, None, None) == -2
+    # a description whose parts would pass 32 bits (every head reads one: stride 0): the workspace stays bounded
+    assert 0 < lib.hv_attn_packed_work_bytes(args(hq=1024, hkv=1024, d=64, nseq=1, total_q=1, total_k=(1 << 30) - 1)) <= 256 << 20
 
 
 def test_fake_kernels():
