@@ -224,22 +224,14 @@ __device__ __forceinline__ void seq_rows(const int* __restrict__ cu, int nseq, l
   if (len < 0) len = 0;
 }
 
-// 16 bytes per lane from memory to LDS at lds + 16 lane, without registers in between.  Inline assembly, so that the
-// compiler does not wait for it before the next LDS read: arrived() does, once per tile.
-__device__ __forceinline__ void dma16(const void* src, unsigned lds) {
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
-#pragma clang diagnostic pop
-}
-// the same from base + off, base the same for the whole wave
+// hv_lds_dma16 from base + off, base the same for the whole wave; arrived() waits for both, once per tile
 __device__ __forceinline__ void dma16_at(const void* wave_base, unsigned off, unsigned lds) {
   const uint64_t b = (uint64_t)wave_base;
   const uint64_t base = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)b) |
                         (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(b >> 32)) << 32;
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
 #pragma clang diagnostic pop
 }
 __device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
@@ -262,7 +254,7 @@ template <typename T, int DP, int ROWS> struct Dma {
     const int i = (wave() * N + n) * 64 + (threadIdx.x & 63), c = ((i % L::CH) ^ L::f(i / L::CH)) * L::EPC;
     return c < d ? c : 0;
   }
-  static __device__ __forceinline__ void send(const T* src, unsigned lds, int n) { dma16(src, lds + (wave() * N + n) * 1024); }
+  static __device__ __forceinline__ void send(const T* src, unsigned lds, int n) { hv_lds_dma16(src, lds + (wave() * N + n) * 1024); }
   __device__ __forceinline__ void issue(unsigned lds) const {
 #pragma unroll
     for (int n = 0; n < N; ++n) send(at[n], lds, n);

@@ -137,6 +137,17 @@ __device__ __forceinline__ float block_sum(float v, float* scratch) {
   return t;
 }
 
+// 16 bytes per lane from memory to LDS at lds + 16 lane (lds: an LDS byte address, the same for the whole wave), without
+// registers in between.  Inline assembly: the compiler does not track it, so it drains no vmcnt before the LDS reads that
+// follow the issue (it cannot tell one buffer's loads from another's reads); the kernel that uses it waits with an explicit
+// vmcnt.  Nor does it see the hazards inside: a load to LDS reads M0, which needs a wait state after the scalar write.
+__device__ __forceinline__ void hv_lds_dma16(const void* src, unsigned lds) {
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
+#pragma clang diagnostic pop
+}
+
 // Device-side bounds checks of the debug build (`make debug` -> libhvs_debug.so, -DHV_DEBUG):
 // a violation prints its file:line and condition; no trap (a trapping wave faults the device
 // for every process on it).  Release builds compile them out.

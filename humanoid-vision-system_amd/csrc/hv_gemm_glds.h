@@ -39,17 +39,6 @@ __device__ __forceinline__ void glds16(const void* src, unsigned char* lds_base)
 #endif
 }
 
-// The same 16-byte LDS-DMA as inline asm (M0 = wave-uniform LDS byte address).  The compiler
-// does not track it, so it does not drain vmcnt before every ds_read that follows the issue
-// (it cannot tell the other buffer's DMA from this buffer's reads); the kernel that uses it
-// waits for its DMAs itself with explicit vmcnt.
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-__device__ __forceinline__ void glds16_asm(const void* src, unsigned lds_addr) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds_addr) : "memory", "m0");
-}
-#pragma clang diagnostic pop
-
 // Implicit-im2col K position of a 64-wide K-tile when conv_c % 64 == 0 (every conv this path
 // serves but the K-tail ones): the tile lies inside ONE tap, so its source offset
 // ((kh * W + kw) * C + ci) is wave-uniform.  Advanced by one K-tile per call instead of
@@ -179,10 +168,10 @@ __global__ void __launch_bounds__(256, (GldsOcc<BM, BN, NS, TRAIN>::value)) gemm
         const int ih = aih[i] + ck.kh, iw = aiw[i] + ck.kw;
         const void* src = ((unsigned)ih < (unsigned)d.conv_h && (unsigned)iw < (unsigned)d.conv_w)
                               ? (const void*)(arow[i] + apix[i] + koff) : (const void*)hv_glds_zero_line;
-        glds16_asm(src, la + i * 1024);
+        hv_lds_dma16(src, la + i * 1024);
       }
 #pragma unroll
-      for (int i = 0; i < BI; ++i) glds16_asm(brow[i] + k, lb + i * 1024);
+      for (int i = 0; i < BI; ++i) hv_lds_dma16(brow[i] + k, lb + i * 1024);
       ck.advance(d);
       return;
     }
@@ -205,13 +194,13 @@ __global__ void __launch_bounds__(256, (GldsOcc<BM, BN, NS, TRAIN>::value)) gemm
           src = k < d.K ? (const void*)(arow[i] + k) : (const void*)hv_glds_zero_line;
         }
       }
-      glds16_asm(src, la + i * 1024);
+      hv_lds_dma16(src, la + i * 1024);
     }
 #pragma unroll
     for (int i = 0; i < BI; ++i) {
       const void* src = brow[i] + k;
       src = k < d.K ? src : (const void*)hv_glds_zero_line;   // K tail (padded conv, or dense K % 64 != 0)
-      glds16_asm(src, lb + i * 1024);
+      hv_lds_dma16(src, lb + i * 1024);
     }
   };
 
@@ -372,7 +361,7 @@ __global__ void __launch_bounds__(256, (GldsOcc<BM, BN, NS, TRAIN>::value)) gemm
 // the barrier that ends the load section preceding a part's first read, every wave waits with a
 // counted vmcnt for its own DMAs of that part (the younger DMAs stay in flight); readers of
 // group 0 are one barrier, of group 1 two barriers past every wave's wait.  DMAs are issued with
-// inline asm (glds16_asm) so the compiler does not drain vmcnt before the ds_reads.
+// inline asm (hv_lds_dma16) so the compiler does not drain vmcnt before the ds_reads.
 constexpr int B256_STAGE = 512 * ROW;       // (256 A + 256 B rows) x 128 B per K-tile buffer
 
 template <int AH, int BH>
@@ -463,7 +452,7 @@ __global__ void __launch_bounds__(512) gemm_pp256_kernel(const hv_gemm_desc d) {
     const int ih = aih[i] + c.kh, iw = aiw[i] + c.kw;
     const void* src = ((unsigned)ih < (unsigned)d.conv_h && (unsigned)iw < (unsigned)d.conv_w)
                           ? (const void*)(arow[i] + apix[i] + koff) : (const void*)hv_glds_zero_line;
-    glds16_asm(src, lds0 + buf * B256_STAGE + arow0[i] * ROW);
+    hv_lds_dma16(src, lds0 + buf * B256_STAGE + arow0[i] * ROW);
   };
 
   auto dma_a = [&](int buf, int kt, int i) {
@@ -484,10 +473,10 @@ __global__ void __launch_bounds__(512) gemm_pp256_kernel(const hv_gemm_desc d) {
         src = arow[i] + k;
       }
     }
-    glds16_asm(src, lds0 + buf * B256_STAGE + arow0[i] * ROW);
+    hv_lds_dma16(src, lds0 + buf * B256_STAGE + arow0[i] * ROW);
   };
   auto dma_b = [&](int buf, int kt, int i) {
-    glds16_asm(brow[i] + kt * 64 + lchunk * 8, lds0 + buf * B256_STAGE + BM * ROW + brow0[i] * ROW);
+    hv_lds_dma16(brow[i] + kt * 64 + lchunk * 8, lds0 + buf * B256_STAGE + BM * ROW + brow0[i] * ROW);
   };
   // the A parts of K-tile kt: TL (rows 0, 1) then B (rows 2, 3); ckn is advanced after part B
   // (this kernel only runs convs with K % 64 == 0, i.e. conv_c % 64 == 0: always the fast path)

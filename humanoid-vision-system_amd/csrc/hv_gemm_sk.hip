@@ -28,13 +28,6 @@ constexpr int SK_ROW = 128;                         // bytes per LDS row (64 bf1
 constexpr int SK_BM = 128, SK_BN = 128;
 constexpr int SK_STAGE = (SK_BM + SK_BN) * SK_ROW;  // 32 KiB per k-tile buffer
 
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-__device__ __forceinline__ void sk_glds16(const void* src, unsigned lds_addr) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds_addr) : "memory", "m0");
-}
-#pragma clang diagnostic pop
-
 // physical column (within a wave's 64) of LDS B row q = b*16 + 4g + j
 __device__ __forceinline__ int sk_perm(int q) { return ((q & 15) >> 2) * 16 + (q >> 4) * 4 + (q & 3); }
 
@@ -89,9 +82,9 @@ __global__ void __launch_bounds__(256, 2) gemm_sk_kernel(const hv_gemm_desc d, i
     const unsigned lb = lds0 + buf * SK_STAGE + SK_BM * SK_ROW + wu * BI * 1024;
     const int k = kt * 64 + lchunk * 8;
 #pragma unroll
-    for (int i = 0; i < AI; ++i) sk_glds16(s.a[i] + k, la + i * 1024);
+    for (int i = 0; i < AI; ++i) hv_lds_dma16(s.a[i] + k, la + i * 1024);
 #pragma unroll
-    for (int i = 0; i < BI; ++i) sk_glds16(s.b[i] + k, lb + i * 1024);
+    for (int i = 0; i < BI; ++i) hv_lds_dma16(s.b[i] + k, lb + i * 1024);
   };
 
   int tile = sk_tile(0, ntiles);
@@ -428,7 +421,7 @@ __global__ void __launch_bounds__(256, 1) gemm_skr_kernel(const hv_gemm_desc d, 
     const int n = min(n0 + (r >> 6) * 64 + sk_perm(r & 63), d.N - 1);
     const unsigned short* bp = (const unsigned short*)d.B + (long)n * d.ldb + lchunk * 8;
 #pragma unroll
-    for (int kt = 0; kt < NK; ++kt) sk_glds16(bp + kt * 64, lds0 + kt * KT + wu * BI * 1024 + i * 1024);
+    for (int kt = 0; kt < NK; ++kt) hv_lds_dma16(bp + kt * 64, lds0 + kt * KT + wu * BI * 1024 + i * 1024);
   }
   // ---- A stream: the DMA cursor (dt-th tile of this workgroup, k-tile dk) runs NS-1 groups ahead
   int dt = 0, dk = 0, g_issued = 0;
@@ -438,14 +431,14 @@ __global__ void __launch_bounds__(256, 1) gemm_skr_kernel(const hv_gemm_desc d, 
 #pragma unroll
     for (int i = 0; i < AI; ++i) {
       const int row = min(tm * SK_BM + (wid * AI + i) * 8 + lrow, d.M - 1);
-      sk_glds16((const unsigned short*)d.A + (long)row * d.lda + dk * 64 + lchunk * 8, la + i * 1024);
+      hv_lds_dma16((const unsigned short*)d.A + (long)row * d.lda + dk * 64 + lchunk * 8, la + i * 1024);
     }
     if constexpr (LN) {
       // row statistics of tile dt (first group only; later groups reload them -- same bytes, so
       // the group size stays fixed): wave w -> {mean, rstd}[w >> 1] rows (w & 1) * 64 .. +63
       const float* src = (wu >> 1) ? d.a_rstd : d.a_mean;
       const int r0 = min(tm * SK_BM + (wu & 1) * 64 + (lane & 15) * 4, d.M - 4 < 0 ? 0 : d.M - 4);
-      sk_glds16(src + r0, lds0 + RCS + (dt & 1) * 4096 + wu * 1024);
+      hv_lds_dma16(src + r0, lds0 + RCS + (dt & 1) * 4096 + wu * 1024);
     }
     ++g_issued;
     if (++dk == NK) { dk = 0; ++dt; }

@@ -136,13 +136,6 @@ constexpr int BK = 128;
 
 __device__ const uint4 zeros = {0, 0, 0, 0};              // what lies behind k
 
-__device__ __forceinline__ void dma16(const void* src, unsigned lds) {
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
-#pragma clang diagnostic pop
-}
-
 // a row's 16-byte chunk c lies at c ^ swz(row): 16 rows' equal chunks are in 256 different bytes
 __device__ __forceinline__ int swz(int row) { return (row >> 1) & 7; }
 
@@ -190,10 +183,10 @@ __global__ void __launch_bounds__(64 * WN * WM, WN * WM / 4) k_linear_fp8(const 
     for (int i = 0; i < D; ++i) {
       const unsigned to = at + (i < DN ? 0 : TN) + place(i) * BK;
       if (whole) {
-        dma16(src[i], to);
+        hv_lds_dma16(src[i], to);
         src[i] += BK;
       } else {
-        dma16(s * BK + ((lane & 7) ^ swz(place(i) + (lane >> 3))) * 16 < p.k ? (const void*)src[i] : (const void*)&zeros, to);
+        hv_lds_dma16(s * BK + ((lane & 7) ^ swz(place(i) + (lane >> 3))) * 16 < p.k ? (const void*)src[i] : (const void*)&zeros, to);
       }
     }
   };

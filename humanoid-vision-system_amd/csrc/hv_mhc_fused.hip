@@ -350,13 +350,6 @@ int launch(const hv_mhc_fused_args* a, hipStream_t s) {
 // iteration ch computes GEMM1 + GELU of chunk ch+1 beside GEMM2 of chunk ch (independent
 // instruction streams the scheduler interleaves: matrix pipe || VALU).  Wc^T goes to LDS whole
 // in the last two iterations (the two stages no chunk needs any more), so GEMM3 runs barrier-free.
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-__device__ __forceinline__ void mhc_glds16(const void* src, unsigned lds_addr) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds_addr) : "memory", "m0");
-}
-#pragma clang diagnostic pop
-
 template <int D, int HD, int TB_, int MINB, int NW_, bool NOMERGE>
 __global__ void __launch_bounds__(64 * NW_, MINB) mhc_fused_pipe_kernel(
     const unsigned short* __restrict__ x, int T, const unsigned short* __restrict__ a1t, const float* __restrict__ c1,
@@ -386,14 +379,14 @@ __global__ void __launch_bounds__(64 * NW_, MINB) mhc_fused_pipe_kernel(
     for (int p0 = 0; p0 < KC * C::CPA; p0 += C::NT) {
       if (p0 + wu * 64 < KC * C::CPA) {
         const int p = p0 + tid, r = p / C::CPA, pc = p % C::CPA;
-        mhc_glds16(a1t + (long)(ch * KC + r) * D + swzA<C::CPA>(r, pc) * 8, sa + (p0 + wu * 64) * 16);
+        hv_lds_dma16(a1t + (long)(ch * KC + r) * D + swzA<C::CPA>(r, pc) * 8, sa + (p0 + wu * 64) * 16);
       }
     }
 #pragma unroll
     for (int p0 = 0; p0 < HD * 4; p0 += C::NT) {
       if (p0 + wu * 64 < HD * 4) {
         const int p = p0 + tid, r = p >> 2, pc = p & 3;
-        mhc_glds16(w2 + (long)r * (2 * HD) + ch * KC + swz64(r, pc) * 8, sw + (p0 + wu * 64) * 16);
+        hv_lds_dma16(w2 + (long)r * (2 * HD) + ch * KC + swz64(r, pc) * 8, sw + (p0 + wu * 64) * 16);
       }
     }
   };
@@ -406,7 +399,7 @@ __global__ void __launch_bounds__(64 * NW_, MINB) mhc_fused_pipe_kernel(
       for (int p0 = 0; p0 < D * 4; p0 += C::NT) {
         if (p0 + wu * 64 < D * 4) {
           const int p = p0 + tid, r = p >> 2, pc = p & 3;
-          mhc_glds16(wct + (long)r * (D + HD) + ks * 32 + swz64(r, pc) * 8, lds0 + wc_chunk(ks) + (p0 + wu * 64) * 16);
+          hv_lds_dma16(wct + (long)r * (D + HD) + ks * 32 + swz64(r, pc) * 8, lds0 + wc_chunk(ks) + (p0 + wu * 64) * 16);
         }
       }
     }
@@ -716,7 +709,7 @@ __global__ void __launch_bounds__(256 * NG, 1) mhc_fused2_kernel(
   const long tg0 = t0 + gq * C::TOKG;                  // first token of this wave's group
   const long tw = t0 + w * C::TW1;                     // first GEMM1 token of this wave
 
-  // weight DMAs as inline asm (mhc_glds16): hipcc does not track them, so it no longer waits
+  // weight DMAs as inline asm (hv_lds_dma16): hipcc does not track them, so it no longer waits
   // vmcnt(0) before every fragment read of the other stages (it cannot tell them apart from the
   // stage being filled); every wait below is explicit
   auto issue_chunk = [&](int ch, int st) {
@@ -725,14 +718,14 @@ __global__ void __launch_bounds__(256 * NG, 1) mhc_fused2_kernel(
     for (int p0 = 0; p0 < KC * C::CPA; p0 += C::NT) {
       if (p0 + wu * 64 < KC * C::CPA) {
         const int p = p0 + tid, r = p / C::CPA, pc = p % C::CPA;
-        mhc_glds16(a1t + (long)(ch * KC + r) * D + swzA<C::CPA>(r, pc) * 8, sa + (p0 + wu * 64) * 16);
+        hv_lds_dma16(a1t + (long)(ch * KC + r) * D + swzA<C::CPA>(r, pc) * 8, sa + (p0 + wu * 64) * 16);
       }
     }
 #pragma unroll
     for (int p0 = 0; p0 < HD * 4; p0 += C::NT) {
       if (p0 + wu * 64 < HD * 4) {
         const int p = p0 + tid, r = p >> 2, pc = p & 3;
-        mhc_glds16(w2 + (long)r * (2 * HD) + ch * KC + swz64(r, pc) * 8, sw + (p0 + wu * 64) * 16);
+        hv_lds_dma16(w2 + (long)r * (2 * HD) + ch * KC + swz64(r, pc) * 8, sw + (p0 + wu * 64) * 16);
       }
     }
   };
@@ -745,7 +738,7 @@ __global__ void __launch_bounds__(256 * NG, 1) mhc_fused2_kernel(
     for (int i = 0; i < C::WPT; ++i) {
       const int p = i * C::NT + tid;
       const int kc = p / (C::DP * 4), r = (p >> 2) % C::DP, pc = p & 3;
-      mhc_glds16(wct + (long)(dp * C::DP + r) * (D + HD) + kc * 32 + swz64(r, pc) * 8, dst + (i * C::NT + wu * 64) * 16);
+      hv_lds_dma16(wct + (long)(dp * C::DP + r) * (D + HD) + kc * 32 + swz64(r, pc) * 8, dst + (i * C::NT + wu * 64) * 16);
     }
   };
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // c1 loads retired before the first DMA
