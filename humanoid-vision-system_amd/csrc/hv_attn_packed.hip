@@ -224,14 +224,15 @@ __device__ __forceinline__ void seq_rows(const int* __restrict__ cu, int nseq, l
   if (len < 0) len = 0;
 }
 
-// hv_lds_dma16 from base + off, base the same for the whole wave; arrived() waits for both, once per tile
+// hv_lds_dma16 from base + off, base the same for the whole wave; arrived() waits for both, once per tile.  The base may come
+// from a lane read right before it (a vector instruction that writes a scalar pair): five wait states before a load takes it.
 __device__ __forceinline__ void dma16_at(const void* wave_base, unsigned off, unsigned lds) {
   const uint64_t b = (uint64_t)wave_base;
   const uint64_t base = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)b) |
                         (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(b >> 32)) << 32;
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
 #pragma clang diagnostic pop
 }
 __device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }

@@ -52,3 +52,18 @@ def test_a_load_to_lds_waits_for_m0():
             writes = [j for j in range(i) if re.match(r"s_\w+\s+m0\b", code[j])]
             assert writes, f"{where}: {x} without its M0"
             assert waits(code[writes[-1] + 1:i]) >= 1, f"{where}: {x} right after the write of M0"
+
+
+def test_a_load_waits_for_its_scalar_address():
+    """A load that takes its base from a scalar pair needs five wait states after a vector instruction (a lane read) wrote the
+    pair.  The operand may come from one, right before the statement, so the statement holds all five."""
+    seen = 0
+    for where, code, operands in statements():
+        for i, x in enumerate(code):
+            if not re.match(r"(global|buffer|flat|scratch)_", x):
+                continue
+            base = [int(n) for n in re.findall(r"%(\d+)", x) if "s" in operands[int(n)]]
+            if base:
+                seen += 1
+                assert waits(code[:i]) >= 5, f"{where}: {x}: {waits(code[:i])} wait states"
+    assert seen
