@@ -824,10 +824,17 @@ def _same_device(what: str, first: Tensor, *others) -> None:
             raise ValueError(f"{what}: tensors on {first.device} and {t.device}")
 
 
+def row_strides(t: Tensor):
+    """(row, head) strides of `t` [rows, heads, d]; 0 where there is one row or one head, whose stride is never used."""
+    row, head, _ = t.stride()
+    return row if t.shape[0] > 1 else 0, head if t.shape[1] > 1 else 0
+
+
 def rows_dense(t: Tensor) -> bool:
     """Whether attention_packed can read `t` [rows, heads, d] in place: last dimension dense, every row
     start on a 16-byte boundary."""
-    row, head, one = t.stride()
+    row, head = row_strides(t)
+    one = t.stride(2)
     return (one == 1 or t.shape[2] == 1) and not (t.data_ptr() | row * t.element_size() | head * t.element_size()) & 15
 
 
@@ -866,9 +873,9 @@ def attn_packed_point(a: L.AttnPackedArgs, q: Tensor, k: Tensor, v: Tensor, cu_q
     """Let the description of a call point at its operands."""
     a.cu_q, a.cu_k = cu_q.data_ptr(), cu_k.data_ptr()
     a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    a.q_row, a.q_head, _ = q.stride()
-    a.k_row, a.k_head, _ = k.stride()
-    a.v_row, a.v_head, _ = v.stride()
+    a.q_row, a.q_head = row_strides(q)
+    a.k_row, a.k_head = row_strides(k)
+    a.v_row, a.v_head = row_strides(v)
 
 
 def attention_packed(q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Optional[Tensor] = None, *,

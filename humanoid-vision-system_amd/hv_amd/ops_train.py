@@ -14,7 +14,7 @@ from torch.autograd.graph import increment_version
 
 from . import _lib as L
 from ._lib import check, dtype_code, ptr, stream_ptr
-from .ops import _contig, _cuda, attn_packed_args, attn_packed_point, f32, norm_operands, on_device, rows_dense
+from .ops import _contig, _cuda, attn_packed_args, attn_packed_point, f32, norm_operands, on_device, row_strides, rows_dense
 from .runtime import options, seed_offset_ptr
 
 Tensor = torch.Tensor
@@ -510,7 +510,7 @@ def attention_packed_backward(q, k, v, cu_q, cu_k, call, out, low, lse, dout, ne
     if dout.shape != q.shape or dout.dtype != q.dtype:
         raise ValueError(f"attention_packed_backward: dout {tuple(dout.shape)} {dout.dtype} is not like q")
     # the kernels address 64 rows of q and dout with 32-bit offsets
-    q, dout = (t.contiguous() if not (rows_dense(t) and max(t.stride()) < 1 << 22) and t.numel() else t
+    q, dout = (t.contiguous() if not (rows_dense(t) and max(row_strides(t)) < 1 << 22) and t.numel() else t
                for t in (q, dout))
     a = L.AttnPackedArgs.from_buffer_copy(call)
     attn_packed_point(a, q, k, v, cu_q, cu_k)
@@ -521,7 +521,7 @@ def attention_packed_backward(q, k, v, cu_q, cu_k, call, out, low, lse, dout, ne
     with on_device(q) as stream:
         a.out, a.out_low, a.lse = out.data_ptr(), ptr(low), lse.data_ptr()
         a.dout = dout.data_ptr()
-        a.do_row, a.do_head, _ = dout.stride()
+        a.do_row, a.do_head = row_strides(dout)
         a.dq, a.dk, a.dv = ptr(dq), ptr(dk), ptr(dv)
         work = torch.empty(lib.hv_attn_packed_backward_work_bytes(C.byref(a)), device=q.device, dtype=torch.uint8)
         a.work = work.data_ptr()

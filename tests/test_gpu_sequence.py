@@ -800,3 +800,24 @@ def test_refusals_with_gpu_tensors(gpu_device):
         ops.attention_packed(q.half(), q.half(), q.half(), cu)
     with pytest.raises(RuntimeError):
         ops.add_rmsnorm(q.cpu(), q.cpu(), torch.ones(32))
+
+
+# ------------------------------------------------------------------------------------------- layouts
+def test_packed_attention_single_row_and_single_head_strides(gpu_device):
+    """One row of a wide buffer, and one head with a meaningless stride: read in place, same bits as dense."""
+    from hv_amd import ops, train_fn
+    g = torch.Generator().manual_seed(17)
+    buf = torch.randn(5, 4 * 32 + 1, generator=g).to(BF).to(gpu_device)
+    q = buf.as_strided((1, 4, 32), (129, 32, 1))
+    k = torch.randn(9, 48, generator=g).to(BF).to(gpu_device).as_strided((9, 1, 32), (48, 5, 1))
+    cq, ck = offsets([1]).to(gpu_device), offsets([9]).to(gpu_device)
+    want = ops.attention_packed(q.clone(memory_format=torch.contiguous_format), k.clone(memory_format=torch.contiguous_format),
+                                k.clone(memory_format=torch.contiguous_format), cq, ck)
+    assert torch.equal(ops.attention_packed(q, k, k, cq, ck), want)
+    leaf = q.detach().requires_grad_(True)
+    out = train_fn.attention_packed(leaf, k, k, cq, ck)
+    do = torch.randn(2, 4, 32, generator=g).to(BF).to(gpu_device).as_strided((1, 4, 32), (1 << 24, 32, 1))
+    (dq,) = torch.autograd.grad(out, leaf, do)
+    val, tol = reference(q, k, k, cq, ck, False, 32 ** -0.5, do)
+    check(out, val["out"], tol["out"], "out")
+    check(dq, val["dq"], tol["dq"], "dq")

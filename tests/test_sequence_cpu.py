@@ -140,3 +140,22 @@ def test_fake_kernels():
         assert c.dtype == torch.float8_e4m3fn and sc.shape == (5,)
         w8, ws = torch.ops.hv.quantize_rows_fp8(torch.empty(7, 64, device=d))
         assert torch.ops.hv.linear_fp8(c, sc, w8, ws).shape == (5, 7)
+
+
+# ------------------------------------------------------------------------------------------- strides and alignment of operands
+def in_place(a, name):
+    """Whether the C entry takes the operand of this description."""
+    head = getattr(a, name + "_head"), getattr(a, name + "_row")
+    return getattr(a, {"do": "dout"}.get(name, name)) % 16 == 0 and all(s * 2 % 16 == 0 for s in head)
+
+
+def test_single_rows_and_heads_have_no_stride(ops):
+    """The stride of a dimension of one element is never used: such operands are read in place."""
+    cu = torch.tensor([0, 1], dtype=torch.int32)
+    q = torch.zeros(5, 4 * 32 + 1, dtype=torch.bfloat16).as_strided((1, 4, 32), (129, 32, 1))
+    k = torch.zeros(5, 2 * 32 + 1, dtype=torch.bfloat16).as_strided((1, 2, 32), (65, 32, 1))
+    a = ops.attn_packed_args(q, k, k, cu, cu, False, None)
+    assert all(in_place(a, n) for n in ("q", "k", "v")) and a.q_head == 32 and a.k == k.data_ptr()
+    one = torch.zeros(6, 48, dtype=torch.bfloat16).as_strided((6, 1, 32), (48, 5, 1))
+    a = ops.attn_packed_args(one, one, one, torch.tensor([0, 6], dtype=torch.int32), torch.tensor([0, 6], dtype=torch.int32), False, None)
+    assert in_place(a, "q") and a.q_row == 48
