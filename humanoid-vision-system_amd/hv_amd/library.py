@@ -254,8 +254,8 @@ def attention_packed(q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Tensor
                      scale: Optional[float] = None) -> Tuple[Tensor, Tensor]:
     """q [rows, heads, d], k / v [rows, kv heads, d], offsets int32 [sequences + 1] -> (out like q, log-sum-exp
     [rows, heads] fp32, not differentiable); see ops.attention_packed."""
-    fit = [t if t.dim() != 3 or ops.rows_dense(t) else t.contiguous() for t in (q, k, v)]
-    return ops.attention_packed(*fit, cu_q, cu_k, causal=causal, scale=scale, return_lse=True)
+    q, k, v = ops.dense_rows(q), ops.dense_rows(k), ops.dense_rows(v)
+    return ops.attention_packed(q, k, v, cu_q, cu_k, causal=causal, scale=scale, return_lse=True)
 
 
 @attention_packed.register_fake

@@ -838,6 +838,12 @@ def rows_dense(t: Tensor) -> bool:
     return (one == 1 or t.shape[2] == 1) and not (t.data_ptr() | row * t.element_size() | head * t.element_size()) & 15
 
 
+def dense_rows(t: Tensor) -> Tensor:
+    """`t` [rows, heads, d] itself where attention_packed can read it in place, else a dense copy (.contiguous() would
+    return a contiguous view that starts off a 16-byte boundary as it is)."""
+    return t if t.dim() != 3 or rows_dense(t) else t.clone(memory_format=torch.contiguous_format)
+
+
 def attn_packed_args(q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Tensor, causal: bool,
                      scale: Optional[float]) -> L.AttnPackedArgs:
     """Check the operands of a packed attention and describe them (hv_attn_packed_args)."""

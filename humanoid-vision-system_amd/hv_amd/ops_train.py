@@ -14,7 +14,8 @@ from torch.autograd.graph import increment_version
 
 from . import _lib as L
 from ._lib import check, dtype_code, ptr, stream_ptr
-from .ops import _contig, _cuda, attn_packed_args, attn_packed_point, f32, norm_operands, on_device, row_strides, rows_dense
+from .ops import (_contig, _cuda, attn_packed_args, attn_packed_point, dense_rows, f32, norm_operands, on_device,
+                  row_strides)
 from .runtime import options, seed_offset_ptr
 
 Tensor = torch.Tensor
@@ -510,8 +511,12 @@ def attention_packed_backward(q, k, v, cu_q, cu_k, call, out, low, lse, dout, ne
     if dout.shape != q.shape or dout.dtype != q.dtype:
         raise ValueError(f"attention_packed_backward: dout {tuple(dout.shape)} {dout.dtype} is not like q")
     # the kernels address 64 rows of q and dout with 32-bit offsets
-    q, dout = (t.contiguous() if not (rows_dense(t) and max(row_strides(t)) < 1 << 22) and t.numel() else t
+    q, dout = (dense_rows(t) if max(row_strides(t)) < 1 << 22 else t.clone(memory_format=torch.contiguous_format)
                for t in (q, dout))
+    # as the forward had them, unless saved-tensor hooks returned them in another layout
+    k, v, lse = dense_rows(k), dense_rows(v), lse.contiguous()
+    out, low = (t if t is None or (t.is_contiguous() and not t.data_ptr() & 15)
+                else t.clone(memory_format=torch.contiguous_format) for t in (out, low))
     a = L.AttnPackedArgs.from_buffer_copy(call)
     attn_packed_point(a, q, k, v, cu_q, cu_k)
     dq = torch.empty(q.shape, device=q.device, dtype=q.dtype) if need_q else None

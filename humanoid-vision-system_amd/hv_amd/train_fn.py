@@ -499,8 +499,8 @@ def attention_packed(q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Option
                      causal: bool = False, scale: Optional[float] = None) -> Tensor:
     """ops.attention_packed, differentiable in q, k and v.  Inputs that the kernels cannot read in place (last
     dimension not dense, rows not 16-byte aligned) are copied."""
-    fit = [t if t.dim() != 3 or ops.rows_dense(t) else t.contiguous() for t in (q, k, v)]
-    return PackedAttentionFn.apply(*fit, cu_q, cu_q if cu_k is None else cu_k, bool(causal), scale)
+    q, k, v = ops.dense_rows(q), ops.dense_rows(k), ops.dense_rows(v)
+    return PackedAttentionFn.apply(q, k, v, cu_q, cu_q if cu_k is None else cu_k, bool(causal), scale)
 
 
 class AddRMSNormFn(torch.autograd.Function):

@@ -821,3 +821,61 @@ def test_packed_attention_single_row_and_single_head_strides(gpu_device):
     val, tol = reference(q, k, k, cq, ck, False, 32 ** -0.5, do)
     check(out, val["out"], tol["out"], "out")
     check(dq, val["dq"], tol["dq"], "dq")
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_packed_attention_contiguous_operands_off_the_boundary(gpu_device, dtype):
+    """Contiguous views that start off a 16-byte boundary, as q, k, v and as the gradient that arrives: the differentiable form
+    and the dispatcher's copy them, same bits as with aligned operands."""
+    from hv_amd import train_fn
+    q, k, v, do, cq, ck = packed_inputs([33, 20], [33, 20], 4, 2, 64, dtype, 18)
+
+    def off(t):
+        view = torch.empty(t.numel() + 3, dtype=t.dtype, device=t.device)[3:].view(t.shape)
+        view.copy_(t)
+        assert view.is_contiguous() and view.data_ptr() % 16
+        return view
+
+    def run(fn, make, do):
+        x = [make(t).requires_grad_(True) for t in (q, k, v)]
+        out = fn(*x)
+        return (out, *torch.autograd.grad(out, x, do))
+
+    import hv_amd  # noqa: F401
+    for fn in (lambda *x: train_fn.attention_packed(*x, cq, ck, causal=True),
+               lambda *x: torch.ops.hv.attention_packed(*x, cq, ck, True)[0]):
+        want = run(fn, torch.clone, do)
+        for a, b in zip(run(fn, off, off(do)), want):
+            assert torch.equal(a, b)
+    # the gradient of one piece of a concatenation
+    x = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    out = train_fn.attention_packed(*x, cq, ck, causal=True)
+    head = torch.ones(3, device=gpu_device, dtype=dtype, requires_grad=True)
+    loss = torch.cat([head, out.flatten()]).float().square().sum()
+    got = torch.autograd.grad(loss, x)
+    want = run(lambda *x: train_fn.attention_packed(*x, cq, ck, causal=True), torch.clone, (2 * out.detach().float()).to(dtype))
+    for a, b in zip(got, want[1:]):
+        assert torch.equal(a, b)
+
+
+def test_packed_attention_saved_tensors_in_another_layout(gpu_device):
+    """Saved-tensor hooks may return operands in another layout: same bits."""
+    from hv_amd import train_fn
+    q, k, v, do, cq, ck = packed_inputs([33, 20], [33, 20], 4, 2, 64, BF, 19)
+
+    def run():
+        x = [t.clone().requires_grad_(True) for t in (q, k, v)]
+        out = train_fn.attention_packed(*x, cq, ck, causal=True)
+        return torch.autograd.grad(out, x, do)
+
+    def odd(t):
+        if t.dim() != 3:
+            return t.t().contiguous().t() if t.dim() == 2 else t
+        wide = torch.zeros(*t.shape[:2], t.shape[2] + 1, dtype=t.dtype, device=t.device)
+        wide[:, :, 1:] = t
+        return wide[:, :, 1:]
+
+    want = run()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, odd):
+        got = run()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

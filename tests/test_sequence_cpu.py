@@ -159,3 +159,57 @@ def test_single_rows_and_heads_have_no_stride(ops):
     one = torch.zeros(6, 48, dtype=torch.bfloat16).as_strided((6, 1, 32), (48, 5, 1))
     a = ops.attn_packed_args(one, one, one, torch.tensor([0, 6], dtype=torch.int32), torch.tensor([0, 6], dtype=torch.int32), False, None)
     assert in_place(a, "q") and a.q_row == 48
+
+
+def odd_views(rows, heads, d, dtype=torch.bfloat16):
+    """Contiguous views off a 16-byte boundary, and single rows / heads whose strides mean nothing."""
+    flat = torch.arange(rows * heads * d + 8, dtype=torch.float32).to(dtype)
+    yield flat[1:1 + rows * heads * d].view(rows, heads, d)
+    yield flat[3:3 + heads * d].view(1, heads, d)
+    yield torch.ones(rows, heads * d + 1, dtype=dtype)[:1, :heads * d].view(1, heads, d)
+    yield torch.ones(rows, heads * d + 3, dtype=dtype)[:, :d].view(rows, 1, d)
+
+def test_operands_off_the_boundary_are_copied(ops, monkeypatch):
+    """The differentiable form hands on operands that the kernels can read, with the same values: .contiguous() alone
+    returns a contiguous view off the boundary as it is."""
+    from hv_amd import train_fn
+    got = []
+    monkeypatch.setattr(train_fn.PackedAttentionFn, "apply", lambda *a: got.append(a))
+    cu = torch.tensor([0, 6], dtype=torch.int32)
+    for t in odd_views(6, 4, 32):
+        train_fn.attention_packed(t, t, t, cu)
+        for x in got.pop()[:3]:
+            assert torch.equal(x, t)
+            a = ops.attn_packed_args(x, x, x, cu, cu, False, None)
+            assert in_place(a, "q")
+
+
+def test_backward_copies_what_it_cannot_read(ops, monkeypatch):
+    """Gradients that arrive as contiguous views off the boundary, far strides of a single row, and operands that saved-tensor
+    hooks returned in another layout."""
+    import contextlib
+    from hv_amd import ops_train as T
+    seen = []
+
+    class Lib:
+        def hv_attn_packed_backward_work_bytes(self, a):
+            return 64
+
+        def hv_attn_packed_backward(self, a, stream):
+            seen.append(T.L.AttnPackedArgs.from_buffer_copy(a._obj))
+            return 0
+
+    monkeypatch.setattr(T.L, "lib", Lib)
+    monkeypatch.setattr(T, "on_device", contextlib.nullcontext)
+    for dout in odd_views(6, 4, 32):
+        n, hq = dout.shape[:2]
+        q = torch.zeros(n, hq, 32, dtype=torch.bfloat16)
+        k = torch.zeros(n, hq * 32 + 1, dtype=torch.bfloat16)[:, :hq * 32].view(n, hq, 32)
+        cu = torch.tensor([0, n], dtype=torch.int32)
+        call = ops.attn_packed_args(q, q, q, cu, cu, False, None)
+        out = torch.zeros(n * hq * 32 + 1, dtype=torch.bfloat16)[1:].view(n, hq, 32)
+        lse = torch.zeros(hq, n).t()
+        T.attention_packed_backward(q, k, k, cu, cu, call, out, torch.zeros_like(q), lse, dout)
+        a = seen.pop()
+        assert all(in_place(a, x) for x in ("q", "k", "v", "do")) and a.out % 16 == 0 and a.out_low % 16 == 0
+        assert a.lse != lse.data_ptr() or lse.is_contiguous()
