@@ -772,7 +772,9 @@ __global__ void __launch_bounds__(NT) k_attn_packed_join(const Args a, int part_
 }
 
 // ------------------------------------------------------------------------------------------------
-// delta_i = dO_i . O_i = sum_j P_ij dP_ij (the mean that the softmax gradient subtracts): 16 lanes per row
+// delta_i = dO_i . O_i = sum_j P_ij dP_ij (the mean that the softmax gradient subtracts): 16 lanes per row.  The log-sum-exp's
+// own gradient has the same form, d lse_i / d S_ij = P_ij, so dS = P o (dP - (delta - dlse)): it is taken off here.  A row
+// that sees no key has none (its lse is the constant -inf).
 template <typename T>
 __global__ void __launch_bounds__(NT) k_attn_packed_delta(const Args a, float* __restrict__ delta) {
   const int c = (threadIdx.x & 15) * 8;                  // d <= 128
@@ -790,7 +792,7 @@ __global__ void __launch_bounds__(NT) k_attn_packed_delta(const Args a, float* _
     }
 #pragma unroll
     for (int x = 8; x > 0; x >>= 1) s += __shfl_xor(s, x, 64);
-    if (c == 0) delta[i] = s;
+    if (c == 0) delta[i] = a.dlse && a.lse[i] != NEG_INF ? s - a.dlse[i] : s;
   }
 }
 

@@ -147,7 +147,7 @@ class AttnPackedArgs(C.Structure):
                 ("scale", f32), ("pad_", i32), ("total_q", i64), ("total_k", i64), ("cu_q", vp), ("cu_k", vp),
                 ("q", vp), ("k", vp), ("v", vp), ("q_row", i64), ("q_head", i64), ("k_row", i64), ("k_head", i64),
                 ("v_row", i64), ("v_head", i64), ("out", vp), ("out_low", vp), ("lse", vp), ("work", vp),
-                ("dout", vp), ("do_row", i64), ("do_head", i64), ("dq", vp), ("dk", vp), ("dv", vp)]
+                ("dout", vp), ("do_row", i64), ("do_head", i64), ("dq", vp), ("dk", vp), ("dv", vp), ("dlse", vp)]
 
 
 _SIGS = {

@@ -253,7 +253,7 @@ attention.register_autograd(_attn_bwd, setup_context=_attn_setup)
 def attention_packed(q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Tensor, causal: bool = False,
                      scale: Optional[float] = None) -> Tuple[Tensor, Tensor]:
     """q [rows, heads, d], k / v [rows, kv heads, d], offsets int32 [sequences + 1] -> (out like q, log-sum-exp
-    [rows, heads] fp32, not differentiable); see ops.attention_packed."""
+    [rows, heads] fp32), both differentiable; see ops.attention_packed."""
     q, k, v = ops.dense_rows(q), ops.dense_rows(k), ops.dense_rows(v)
     return ops.attention_packed(q, k, v, cu_q, cu_k, causal=causal, scale=scale, return_lse=True)
 
@@ -270,10 +270,11 @@ def _attn_packed_setup(ctx, inputs, output):
 
 
 def _attn_packed_bwd(ctx, do, dlse):
-    from .train_fn import attention_packed as packed
+    from .train_fn import PackedAttentionFn
     q, k, v, cu_q, cu_k = ctx.saved_tensors
     causal, scale = ctx.meta
-    g = _grad_of(lambda a, b, c: packed(a, b, c, cu_q, cu_k, causal=causal, scale=scale), [q, k, v], [do])
+    fn = lambda *x: PackedAttentionFn.apply(*(ops.dense_rows(t) for t in x), cu_q, cu_k, causal, scale)    # noqa: E731
+    g = _grad_of(fn, [q, k, v], [do, dlse])
     return g[0], g[1], g[2], None, None, None, None
 
 

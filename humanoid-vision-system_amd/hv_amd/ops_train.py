@@ -506,10 +506,15 @@ def attention_packed_train(q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: 
 
 
 def attention_packed_backward(q, k, v, cu_q, cu_k, call, out, low, lse, dout, need_q: bool = True,
-                              need_kv: bool = True):
-    """(dq, dk, dv) of attention_packed_train, dense; the ones that are not needed are None."""
+                              need_kv: bool = True, dlse: Optional[Tensor] = None):
+    """(dq, dk, dv) of attention_packed_train, dense; the ones that are not needed are None.  dlse: the gradient of the
+    log-sum-exp, fp32 [rows, heads]."""
     if dout.shape != q.shape or dout.dtype != q.dtype:
         raise ValueError(f"attention_packed_backward: dout {tuple(dout.shape)} {dout.dtype} is not like q")
+    if dlse is not None:
+        if dlse.shape != lse.shape or dlse.dtype != torch.float32:
+            raise ValueError(f"attention_packed_backward: dlse {tuple(dlse.shape)} {dlse.dtype} is not like lse")
+        dlse = dlse.contiguous()
     # the kernels address 64 rows of q and dout with 32-bit offsets
     q, dout = (dense_rows(t) if max(row_strides(t)) < 1 << 22 else t.clone(memory_format=torch.contiguous_format)
                for t in (q, dout))
@@ -527,7 +532,7 @@ def attention_packed_backward(q, k, v, cu_q, cu_k, call, out, low, lse, dout, ne
         a.out, a.out_low, a.lse = out.data_ptr(), ptr(low), lse.data_ptr()
         a.dout = dout.data_ptr()
         a.do_row, a.do_head = row_strides(dout)
-        a.dq, a.dk, a.dv = ptr(dq), ptr(dk), ptr(dv)
+        a.dq, a.dk, a.dv, a.dlse = ptr(dq), ptr(dk), ptr(dv), ptr(dlse)
         work = torch.empty(lib.hv_attn_packed_backward_work_bytes(C.byref(a)), device=q.device, dtype=torch.uint8)
         a.work = work.data_ptr()
         check(lib.hv_attn_packed_backward(C.byref(a), stream), "hv_attn_packed_backward")

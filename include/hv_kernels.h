@@ -771,11 +771,12 @@ typedef struct hv_attn_packed_args {
   const void* dout;
   long do_row, do_head;
   void *dq, *dk, *dv;
+  const float* dlse;            /* [total_q, hq] gradient of lse (NULL: none); rows whose lse is -inf take none */
 } hv_attn_packed_args;
 size_t hv_attn_packed_args_bytes(void);   /* sizeof, for bindings */
 size_t hv_attn_packed_work_bytes(const hv_attn_packed_args* a);
 int hv_attn_packed(const hv_attn_packed_args* a, hv_stream_t stream);
-/* dq (NULL: not wanted), dk and dv (both or neither) from q, k, v, out (+ out_low), lse and dout; gradients of a
+/* dq (NULL: not wanted), dk and dv (both or neither) from q, k, v, out (+ out_low), lse, dout and dlse; gradients of a
    shared key / value head are summed over its query heads in fp32; rows of no sequence get 0.  No atomics: equal
    calls give equal bits.  64 rows of q and dout lie within 2^29 elements. */
 size_t hv_attn_packed_backward_work_bytes(const hv_attn_packed_args* a);

@@ -879,3 +879,85 @@ def test_packed_attention_saved_tensors_in_another_layout(gpu_device):
     with torch.autograd.graph.saved_tensors_hooks(lambda t: t, odd):
         got = run()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ------------------------------------------------------------------------------------------- the log-sum-exp's gradient
+def lse_gradient(q, k, cu_q, cu_k, causal, scale, dlse):
+    """What a gradient of the log-sum-exp adds to dq and dk, in 64 bits, and its bounds.  d lse_i / d s_ij = p_ij, so
+    dS_ij = p_ij dlse_i: rounded to the operand type (u), weights off by 4 `off` as in reference(), one fp32 subtraction
+    from the row mean (2 e |dlse|), sums as there, and the result's rounding by the triangle inequality."""
+    u = unit(q.dtype)
+    q, k, dlse = (t.detach().cpu().double() for t in (q, k, dlse))
+    d, grp = q.shape[2], q.shape[1] // k.shape[1]
+    val = {"dq": torch.zeros_like(q), "dk": torch.zeros_like(k)}
+    tol = {n: torch.zeros_like(t) for n, t in val.items()}
+    for s in range(len(cu_q) - 1):
+        a0, a1, b0, b1 = (int(x) for x in (cu_q[s], cu_q[s + 1], cu_k[s], cu_k[s + 1]))
+        lq, lk = a1 - a0, b1 - b0
+        if lq == 0 or lk == 0:
+            continue
+        see = torch.arange(lk)[None, :] <= torch.arange(lq)[:, None] + (lk - lq if causal else lk)
+        for h in range(q.shape[1]):
+            qs, ks = q[a0:a1, h], k[b0:b1, h // grp]
+            p = torch.softmax((qs @ ks.t() * scale).masked_fill(~see, -float("inf")), -1).nan_to_num(0.0)
+            big = torch.where(see, qs.abs() @ ks.abs().t() * scale, torch.zeros(1, dtype=torch.float64))
+            off = ((d + 4) * E * big + 8 * E * (1 + big)).max(-1, keepdim=True).values + (lk + 8) * E
+            ds = p * dlse[a0:a1, h].where(see.any(-1), torch.zeros(1, dtype=torch.float64))[:, None]
+            eS = (u + 4 * off + 2 * E) * ds.abs()
+            val["dq"][a0:a1, h] = scale * ds @ ks
+            tol["dq"][a0:a1, h] = scale * (eS @ ks.abs() + (lk + 4) * E * (ds.abs() @ ks.abs()))
+            val["dk"][b0:b1, h // grp] += scale * ds.t() @ qs
+            tol["dk"][b0:b1, h // grp] += scale * (eS.t() @ qs.abs() + (lq * q.shape[1] + 4) * E * (ds.abs().t() @ qs.abs()))
+    for n in val:
+        tol[n] += u * val[n].abs()
+    return val, tol
+
+
+@pytest.mark.parametrize("name", ["one", "ragged", "blind", "cross", "step"])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype,hq,hkv,d", [(BF, 4, 2, 64), (F32, 3, 1, 32)])
+def test_packed_attention_gradient_of_the_log_sum_exp(gpu_device, name, causal, dtype, hq, hkv, d):
+    """Both outputs of hv::attention_packed in a loss, and each alone; rows that see no key take nothing, whatever arrives."""
+    import hv_amd  # noqa: F401
+    lq, lk = lengths(name)
+    q, k, v, do, cq, ck = packed_inputs(lq, lk, hq, hkv, d, dtype, 23, before=2, spare=3)
+    x = [t.requires_grad_(True) for t in (q, k, v)]
+    out, lse = torch.ops.hv.attention_packed(*x, cq, ck, causal)
+    dlse = torch.randn(lse.shape, generator=torch.Generator().manual_seed(24)).to(gpu_device)
+    dlse[torch.isinf(lse)] = float("nan")
+    val, tol = reference(q, k, v, cq, ck, causal, d ** -0.5, do)
+    vl, tl = lse_gradient(q, k, cq, ck, causal, d ** -0.5, dlse)
+    both = torch.autograd.grad((out, lse), x, (do, dlse), retain_graph=True)
+    for n, t in zip(("dq", "dk"), both):
+        check(t, val[n] + vl[n], tol[n] + tl[n], n)
+    check(both[2], val["dv"], tol["dv"], "dv")
+    alone = torch.autograd.grad(lse, x, dlse, retain_graph=True, allow_unused=True)
+    for n, t in zip(("dq", "dk"), alone):
+        check(t, vl[n], tl[n], n + " of lse alone")
+    assert alone[2] is None or (alone[2] == 0).all()
+    for n, t in zip(("dq", "dk", "dv"), torch.autograd.grad(out, x, do)):
+        check(t, val[n], tol[n], n + " of out alone")
+
+
+def test_packed_attention_lse_gradient_against_differences(gpu_device):
+    """As the differences of the output above: h = 2^-6 leaves h^2 / 6 times a third derivative of order 1 and
+    2^-24 |f| / h, both below 1e-3 of the slope's scale."""
+    import hv_amd  # noqa: F401
+    from hv_amd import ops
+    q, k, v, _, cq, ck = packed_inputs([20, 41], [33, 41], 4, 2, 32, F32, 25)
+    x = [(t * 0.5).requires_grad_(True) for t in (q, k)]
+    _, lse = torch.ops.hv.attention_packed(*x, v, cq, ck, True)
+    g = torch.Generator().manual_seed(26)
+    w = torch.randn(lse.shape, generator=g).to(gpu_device)
+    grads = torch.autograd.grad(lse, x, w)
+    h = 2.0 ** -6
+    for i, grad in enumerate(grads):
+        t = torch.randn(grad.shape, generator=g).to(gpu_device)
+        t /= t.norm()
+        f = []
+        for sign in (1, -1):
+            y = [a.detach() for a in x]
+            y[i] = y[i] + sign * h * t
+            f.append((ops.attention_packed(*y, v, cq, ck, causal=True, return_lse=True)[1].double() * w.double()).sum())
+        slope, want = ((f[0] - f[1]) / (2 * h)).item(), (grad.double() * t.double()).sum().item()
+        assert abs(slope - want) <= 1e-3 * grad.double().norm().item(), (i, slope, want)

@@ -174,7 +174,7 @@ def test_operands_off_the_boundary_are_copied(ops, monkeypatch):
     returns a contiguous view off the boundary as it is."""
     from hv_amd import train_fn
     got = []
-    monkeypatch.setattr(train_fn.PackedAttentionFn, "apply", lambda *a: got.append(a))
+    monkeypatch.setattr(train_fn.PackedAttentionFn, "apply", lambda *a: got.append(a) or (None, None))
     cu = torch.tensor([0, 6], dtype=torch.int32)
     for t in odd_views(6, 4, 32):
         train_fn.attention_packed(t, t, t, cu)
@@ -213,3 +213,40 @@ def test_backward_copies_what_it_cannot_read(ops, monkeypatch):
         a = seen.pop()
         assert all(in_place(a, x) for x in ("q", "k", "v", "do")) and a.out % 16 == 0 and a.out_low % 16 == 0
         assert a.lse != lse.data_ptr() or lse.is_contiguous()
+
+
+def test_dispatcher_gradient_carries_the_log_sum_exp(ops, monkeypatch):
+    """A gradient of the second output reaches the backward kernel: it is an output like the first."""
+    import contextlib
+    import types
+    from hv_amd import library, ops_train as T
+    seen = []
+
+    class Lib:
+        def hv_attn_packed_work_bytes(self, a):
+            return 0
+
+        def hv_attn_packed(self, a, stream):
+            return 0
+
+        def hv_attn_packed_backward_work_bytes(self, a):
+            return 64
+
+        def hv_attn_packed_backward(self, a, stream):
+            a = a._obj
+            seen.append((C.c_float * 24).from_address(a.dlse)[:] if a.dlse else None)
+            return 0
+
+    monkeypatch.setattr(T.L, "lib", Lib)
+    monkeypatch.setattr(T, "on_device", contextlib.nullcontext)
+    q, cu = torch.zeros(6, 4, 32, dtype=torch.bfloat16), torch.tensor([0, 6], dtype=torch.int32)
+    ctx = types.SimpleNamespace(saved_tensors=(q, q, q, cu, cu), meta=(True, None))
+    dlse = torch.arange(24, dtype=torch.float32).view(6, 4)
+    library._attn_packed_bwd(ctx, torch.zeros_like(q), dlse)
+    assert seen.pop() == dlse.flatten().tolist()
+    library._attn_packed_bwd(ctx, torch.zeros_like(q), dlse.t().contiguous().t())
+    assert seen.pop() == dlse.flatten().tolist()
+    library._attn_packed_bwd(ctx, torch.zeros_like(q), None)
+    assert seen.pop() is None
+    library._attn_packed_bwd(ctx, None, dlse)                       # the log-sum-exp alone
+    assert seen.pop() == dlse.flatten().tolist()
