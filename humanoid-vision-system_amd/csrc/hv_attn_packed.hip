@@ -1119,9 +1119,9 @@ size_t part_rows(const hv_attn_packed_args& a, long n) { return (size_t)((a.tota
 // rows, us: 1 x 4 rows, 4096 keys of 128: 69 / 14; 8 x 4, 1024: 22 / 15; 64 x 4, 1024: 47 / 45; 8 x 64, 1024: 21 / 26; 1 x 64,
 // 4096: 59 / 22; 64 columns: 64 x 1, 512: 12 / 18; 8 x 64, 1024: 13 / 19; 1 x 128, 4096: 35 / 25.
 // Parts are sized for about two blocks per CU (12 queries against 85 056 keys, 8 heads: 78 us, four 85 us), 128 keys (one
-// slab per wave) at least.
+// slab per wave) at least.  The join has a wave per (token, head): the tile form also where those pass a grid's 2^32 threads.
 int part_keys(const hv_attn_packed_args& a) {
-  if (a.nseq == 0 || a.total_q == 0 || a.total_k == 0) return 0;
+  if (a.nseq == 0 || a.total_q == 0 || a.total_k == 0 || a.total_q * a.hq > (1L << 26) - 4) return 0;
   const long tiles = (a.total_q * (a.hq / a.hkv) + 32L * a.nseq - 1) / (32L * a.nseq);      // of 32 rows a sequence
   if (tiles > 8 || a.total_k < 512 * (tiles + 1) * a.nseq) return 0;
   const long n0 = min((a.total_k * a.hkv + 511) / 512, a.total_k);      // <= 2^30, also with more than 512 heads
@@ -1129,7 +1129,7 @@ int part_keys(const hv_attn_packed_args& a) {
   // longer parts where the workspace (the number of parts that one sequence with all the keys would have, for every row)
   // would pass 256 MiB: many sequences, which are short against all keys together
   while (n < a.total_k && part_rows(a, n) * (a.d + 4) * sizeof(float) > (256u << 20)) n *= 2;
-  return (int)n;
+  return tile_bound(a.total_k, a.nseq, 1, (int)n) * a.hkv < MAX_BLOCKS ? (int)n : 0;
 }
 
 template <typename T, int DP> void launch_keys(const Args& a, int n, hipStream_t s) {
@@ -1213,8 +1213,7 @@ extern "C" int hv_attn_packed(const hv_attn_packed_args* a, hv_stream_t stream) 
   hipStream_t s = (hipStream_t)stream;
   const int n = part_keys(*a);
   if (n) {
-    if (a->work == nullptr || ((uintptr_t)a->work & 15) || tile_bound(a->total_k, a->nseq, 1, n) * a->hkv >= MAX_BLOCKS)
-      return HV_EINVAL;
+    if (a->work == nullptr || ((uintptr_t)a->work & 15)) return HV_EINVAL;
     HV_DISPATCH(a->dtype, HV_HEAD_DIM(a->d, launch_keys, Args(*a), n, s));
   } else
     HV_DISPATCH(a->dtype, HV_HEAD_DIM(a->d, launch_forward, Args(*a), s));

@@ -753,7 +753,9 @@ int hv_stability_stats(int dtype, const void* x_in, const void* x_out, int rows,
  * value head h / (hq / hkv).  Offsets are read on the device and clamped to the tensors.
  * Rows may lie apart (*_row, *_head: strides in elements, 0 or more; the last dimension is dense); every
  * row start must be 16-byte aligned.  Inside a sequence the values are finite (a hidden key is multiplied
- * by 0); what other rows hold does not matter.  out, out_low, dq, dk, dv are dense [rows, heads, d]. */
+ * by 0); what other rows hold does not matter.  out, out_low, dq, dk, dv are dense [rows, heads, d].
+ * Sizes of one call: (total_q (hq / hkv) / 64 + nseq + 2) hkv below 2^24, for dk and dv (total_k / 64 + nseq + 2) hkv
+ * below 2^21; more is HV_EUNSUPPORTED. */
 typedef struct hv_attn_packed_args {
   int dtype, hq, hkv, d;        /* HV_F32 / HV_BF16; hq % hkv == 0, hq / hkv <= 64, hq <= 1024; d % 8 == 0, d <= 128 */
   int nseq, causal;

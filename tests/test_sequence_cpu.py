@@ -250,3 +250,18 @@ def test_dispatcher_gradient_carries_the_log_sum_exp(ops, monkeypatch):
     assert seen.pop() is None
     library._attn_packed_bwd(ctx, None, dlse)                       # the log-sum-exp alone
     assert seen.pop() == dlse.flatten().tolist()
+
+
+def test_few_rows_form_only_where_its_grid_fits():
+    """The join has a wave per (token, head): 2^26 of them and more are past a grid's 2^32 threads, the tile form takes them
+    (no workspace)."""
+    from hv_amd import _lib as L
+
+    def work(total_q):
+        a = L.AttnPackedArgs()
+        for n, v in dict(dtype=1, hq=64, hkv=4, d=8, nseq=(1 << 20) - 1, scale=0.5, total_q=total_q, total_k=(1 << 30) - 1).items():
+            setattr(a, n, v)
+        return L.lib().hv_attn_packed_work_bytes(C.byref(a))
+
+    assert work((1 << 19) - 1) > 0
+    assert work((1 << 20) - 1) > 0 and work(1 << 20) == 0
