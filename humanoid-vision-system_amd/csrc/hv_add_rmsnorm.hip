@@ -88,7 +88,7 @@ struct NormArgs {
   const void* x;
   long ldx;
   const void* residual;
-  long rows;
+  long rows, first;               // this launch: rows first .. rows - 1
   int cols, x_dtype, r_dtype;
   float eps;
   const float* w;                 // null: rows are quantised as they are
@@ -105,7 +105,7 @@ template <typename TY, int VW, int TPR, int V>
 __global__ void __launch_bounds__(threads_of<TPR>()) k_add_rmsnorm(const NormArgs a) {
   __shared__ float red[16];
   constexpr int RPB = threads_of<TPR>() / TPR;           // rows of a block
-  const long row = (long)blockIdx.x * RPB + threadIdx.x / TPR;
+  const long row = a.first + (long)blockIdx.x * RPB + threadIdx.x / TPR;
   const int t = threadIdx.x % TPR;
   if (row >= a.rows) return;                             // whole waves, and whole blocks where the row spans waves
   const long base = row * a.cols;
@@ -323,16 +323,19 @@ constexpr int MAX_COLS = 32768;
     }                                                      \
   } while (0)
 
-template <typename TY> int launch_norm(const NormArgs& a, bool wide, hipStream_t s) {
+constexpr long LAUNCH_ROWS = 1L << 21;                   // of one launch: a grid stays below 2^32 threads
+
+template <typename TY> int launch_norm(NormArgs a, bool wide, hipStream_t s) {
 #define HV_NORM_CALL(VW, TPR, V)                                                                    \
-  k_add_rmsnorm<TY, VW, TPR, V><<<hv_cdiv(a.rows, threads_of<TPR>() / TPR), threads_of<TPR>(), 0, s>>>(a)
-  HV_ROW_SHAPE(a.cols, wide, HV_NORM_CALL);
+  k_add_rmsnorm<TY, VW, TPR, V><<<hv_cdiv(a.rows - a.first, threads_of<TPR>() / TPR), threads_of<TPR>(), 0, s>>>(a)
+  for (const long rows = a.rows; a.first < rows; a.first += LAUNCH_ROWS) {
+    a.rows = rows < a.first + LAUNCH_ROWS ? rows : a.first + LAUNCH_ROWS;
+    HV_ROW_SHAPE(a.cols, wide, HV_NORM_CALL);
+    HV_CHECK_LAUNCH();
+  }
 #undef HV_NORM_CALL
-  HV_CHECK_LAUNCH();
   return HV_OK;
 }
-
-constexpr long MAX_ROWS = 1L << 23;                      // a grid stays below 2^32 threads
 
 bool a16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
@@ -351,11 +354,11 @@ extern "C" int hv_add_rmsnorm(int x_dtype, const void* x, int r_dtype, const voi
                               float* rstd, hv_stream_t stream) {
   if (!is_float(x_dtype) || (residual && !is_float(r_dtype)) || rows < 0 || cols <= 0 || !(eps >= 0.f)) return HV_EINVAL;
   if (!(is_float(y_dtype) || y_dtype == HV_E4M3)) return HV_EINVAL;
-  if (cols > MAX_COLS || rows > MAX_ROWS) return HV_EUNSUPPORTED;
+  if (cols > MAX_COLS) return HV_EUNSUPPORTED;
   if (rows == 0) return HV_OK;
   if (!x || !scale || !y || (residual && !sum) || (y_dtype == HV_E4M3 && !y_scale)) return HV_EINVAL;
   const bool wide = cols % 8 == 0 && a16(x) && a16(residual) && a16(scale) && a16(sum) && a16(y);
-  const NormArgs a{x, cols, residual, rows, cols, x_dtype, r_dtype, eps, scale, sum, y, y_scale, rstd};
+  const NormArgs a{x, cols, residual, rows, 0, cols, x_dtype, r_dtype, eps, scale, sum, y, y_scale, rstd};
   hipStream_t s = (hipStream_t)stream;
   hv_diag_count(HV_KF_ADD_RMSNORM);
   if (y_dtype == HV_E4M3) return launch_norm<unsigned char>(a, wide, s);
@@ -366,11 +369,11 @@ extern "C" int hv_add_rmsnorm(int x_dtype, const void* x, int r_dtype, const voi
 extern "C" int hv_quantize_rows_fp8(int dtype, const void* x, long ld, long rows, int cols, void* codes, float* scale,
                                     hv_stream_t stream) {
   if (!is_float(dtype) || rows < 0 || cols <= 0 || ld < cols) return HV_EINVAL;
-  if (cols > MAX_COLS || rows > MAX_ROWS) return HV_EUNSUPPORTED;
+  if (cols > MAX_COLS) return HV_EUNSUPPORTED;
   if (rows == 0) return HV_OK;
   if (!x || !codes || !scale) return HV_EINVAL;
   const bool wide = cols % 8 == 0 && ld % 8 == 0 && a16(x) && ((uintptr_t)codes & 7) == 0;
-  const NormArgs a{x, ld, nullptr, rows, cols, dtype, dtype, 0.f, nullptr, nullptr, codes, scale, nullptr};
+  const NormArgs a{x, ld, nullptr, rows, 0, cols, dtype, dtype, 0.f, nullptr, nullptr, codes, scale, nullptr};
   return launch_norm<unsigned char>(a, wide, (hipStream_t)stream);
 }
 
@@ -384,7 +387,7 @@ extern "C" int hv_add_rmsnorm_backward(int x_dtype, const void* x, int r_dtype, 
                                        hv_stream_t stream) {
   if (!is_float(x_dtype) || !is_float(r_dtype) || !is_float(dy_dtype) || (dx && !is_float(dx_dtype)) || rows < 0 || cols <= 0)
     return HV_EINVAL;
-  if (cols > MAX_COLS || rows > MAX_ROWS) return HV_EUNSUPPORTED;
+  if (cols > MAX_COLS) return HV_EUNSUPPORTED;
   if (!dscale || (rows > 0 && (!x || !rstd || !scale || !dy || !work))) return HV_EINVAL;
   hipStream_t s = (hipStream_t)stream;
   const int nb = rows > 0 ? norm_blocks(rows, cols) : 0;

@@ -961,3 +961,25 @@ def test_packed_attention_lse_gradient_against_differences(gpu_device):
             f.append((ops.attention_packed(*y, v, cq, ck, causal=True, return_lse=True)[1].double() * w.double()).sum())
         slope, want = ((f[0] - f[1]) / (2 * h)).item(), (grad.double() * t.double()).sum().item()
         assert abs(slope - want) <= 1e-3 * grad.double().norm().item(), (i, slope, want)
+
+
+# ------------------------------------------------------------------------------------------- sizes of one call
+def test_norm_and_row_codes_of_many_rows(gpu_device):
+    """More rows than one launch has: every row as in a call of its own."""
+    from hv_amd import ops
+    g = torch.Generator().manual_seed(30)
+    rows, part = (1 << 23) + 5, slice((1 << 21) - 3, (1 << 21) + 3)
+    x = torch.randn(1 << 16, 8, generator=g).to(BF).to(gpu_device).repeat(129, 1)[:rows]
+    r, w = x.flip(0), torch.randn(8, generator=g).to(gpu_device)
+    got = (*ops.add_rmsnorm(x, r, w), *ops.add_rmsnorm_fp8(x, r, w), *ops.quantize_rows_fp8(x))
+    for s in (slice(0, 7), part, slice(rows - 9, rows)):
+        want = (*ops.add_rmsnorm(x[s], r[s], w), *ops.add_rmsnorm_fp8(x[s], r[s], w), *ops.quantize_rows_fp8(x[s]))
+        for a, b in zip(got, want):
+            assert torch.equal(a[s].float(), b.float())
+    from hv_amd import train_fn
+    leaf = [t.requires_grad_(True) for t in (x, r, w)]
+    dy = x.detach()
+    dx, _, dw = torch.autograd.grad(train_fn.add_rmsnorm(*leaf)[0], leaf, dy)
+    s = slice(rows - 9, rows)
+    (tail,) = torch.autograd.grad(train_fn.add_rmsnorm(x[s], r[s], w)[0], x, dy[s])
+    assert torch.equal(dx[s], tail[s])
