@@ -303,7 +303,6 @@ template <typename T, int WN, int WM, int NT_, int MT_, int STAGES> int launch_t
 
 template <typename T> int launch_rows(const LinArgs& p, hipStream_t s) {
   const dim3 g(hv_cdiv(p.n, 16), p.m <= 64 ? 1 : hv_cdiv(p.m, 64));
-  if (g.y > 65535) return HV_EUNSUPPORTED;
   if (p.m <= 16) k_linear_fp8_rows<T, 1><<<g, 512, 0, s>>>(p);
   else if (p.m <= 32) k_linear_fp8_rows<T, 2><<<g, 512, 0, s>>>(p);
   else k_linear_fp8_rows<T, 4><<<g, 512, 0, s>>>(p);
@@ -315,12 +314,13 @@ template <typename T> int launch_rows(const LinArgs& p, hipStream_t s) {
 // Measured, us per 128 codes: few-rows form 0.13 / 0.2 / 0.3 (16 / 32 / 64 rows a block), tiles of 64 / 128 / 256: 0.43 /
 // 0.93 / 1.4 (k = 8192, 4096 outputs: 64 rows 22.0 / 29.5 / 60.3 / 61.5 us, 256 rows 81.1 / 30.5 / 61.0 / 91.1, 1024 rows
 // 315 / 110 / 64.4 / 92.3, 4096 rows 1249 / 427 / 238 / 118; k = 1024, 8192 outputs: 128 rows 16.9 / 6.8 / 11.9 / 13.8).
+// The few-rows form has its 64-row blocks in the grid's second dimension, which ends at 65535.
 template <typename T> int launch(const LinArgs& p, hipStream_t s) {
   auto rounds = [&](long blocks) { return (double)((blocks + 255) / 256); };
   auto tiles = [&](int b) { return rounds((long)hv_cdiv(p.m, b) * hv_cdiv(p.n, b)); };
   const double few = rounds((long)hv_cdiv(p.n, 16) * hv_cdiv(p.m, 64)) * (p.m <= 16 ? 0.13 : p.m <= 32 ? 0.2 : 0.3);
   const double t64 = tiles(64) * 0.43, t128 = tiles(128) * 0.93, t256 = tiles(256) * 1.4;
-  if (few <= t64 && few <= t128 && few <= t256) return launch_rows<T>(p, s);
+  if (few <= t64 && few <= t128 && few <= t256 && hv_cdiv(p.m, 64) <= 65535) return launch_rows<T>(p, s);
   if (t64 <= t128 && t64 <= t256) return launch_tiles<T, 2, 2, 1, 1, 6>(p, s);
   return t128 <= t256 ? launch_tiles<T, 2, 2, 2, 2, 3>(p, s) : launch_tiles<T, 2, 4, 4, 2, 2>(p, s);
 }

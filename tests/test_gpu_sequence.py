@@ -983,3 +983,20 @@ def test_norm_and_row_codes_of_many_rows(gpu_device):
     s = slice(rows - 9, rows)
     (tail,) = torch.autograd.grad(train_fn.add_rmsnorm(x[s], r[s], w)[0], x, dy[s])
     assert torch.equal(dx[s], tail[s])
+
+
+def test_linear_fp8_of_many_rows_and_few_outputs(gpu_device):
+    """More rows than the few-rows form has blocks for."""
+    from hv_amd import ops
+    g = torch.Generator().manual_seed(31)
+    m = 64 * 65536 + 5
+    a, sa = ops.quantize_rows_fp8(torch.randn(1 << 12, 16, generator=g).to(gpu_device))
+    a, sa = a.view(torch.uint8).repeat(1025, 1)[:m].view(torch.float8_e4m3fn), sa.repeat(1025)[:m]
+    w, sw = ops.quantize_rows_fp8(torch.randn(16, 16, generator=g).to(gpu_device))
+    y = ops.linear_fp8(a, sa, w, sw)
+    small = ops.linear_fp8(a[:1 << 12], sa[:1 << 12], w, sw)
+    A, W = (c.float().cpu().double() * s.cpu().double()[:, None] for c, s in ((a[:1 << 12], sa[:1 << 12]), (w, sw)))
+    check(small, A @ W.t(), unit(BF) * (A @ W.t()).abs() * 1.01 + fp8_loss(A, W), "one repetition")
+    for s in (slice(0, 1 << 12), slice(m - 5 - (1 << 12), m - 5)):
+        check(y[s], A @ W.t(), unit(BF) * (A @ W.t()).abs() * 1.01 + fp8_loss(A, W), "rows")
+    check(y[m - 5:], (A @ W.t())[:5], (unit(BF) * (A @ W.t()).abs() * 1.01 + fp8_loss(A, W))[:5], "last rows")
