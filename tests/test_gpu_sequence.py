@@ -1000,3 +1000,100 @@ def test_linear_fp8_of_many_rows_and_few_outputs(gpu_device):
     for s in (slice(0, 1 << 12), slice(m - 5 - (1 << 12), m - 5)):
         check(y[s], A @ W.t(), unit(BF) * (A @ W.t()).abs() * 1.01 + fp8_loss(A, W), "rows")
     check(y[m - 5:], (A @ W.t())[:5], (unit(BF) * (A @ W.t()).abs() * 1.01 + fp8_loss(A, W))[:5], "last rows")
+
+
+# ------------------------------------------------------------------------------------------- every form, in its steady state
+def kernels_of(fn, *names):
+    """Names of the kernels that fn() launches, of those that contain one of `names`."""
+    from torch.profiler import ProfilerActivity, profile
+    fn()
+    torch.cuda.synchronize()
+    with profile(activities=[ProfilerActivity.CUDA]) as prof:
+        fn()
+        torch.cuda.synchronize()
+    return {e.key for e in prof.key_averages() if any(n in e.key for n in names)}
+
+
+# (m, n, k, tile's block shape in the kernel's name): over twice as many stages of 128 codes as the form has buffers (6 / 3 / 2),
+# whole ones and a part at the end, edges in m and n
+LONG_LINEAR = [(700, 700, 2064, "2, 2, 1, 1, 6"), (520, 1000, 1792, "2, 2, 1, 1, 6"), (1100, 2100, 1040, "2, 2, 2, 2, 3"),
+               (1025, 2050, 2064, "2, 2, 2, 2, 3"), (1030, 4100, 1040, "2, 4, 4, 2, 2"), (2000, 2100, 784, "2, 4, 4, 2, 2")]
+
+
+@pytest.mark.parametrize("m,n,k,tile", LONG_LINEAR)
+def test_linear_fp8_long_k(gpu_device, m, n, k, tile):
+    """The tile forms with their buffers in rotation: exact sums (codes as in test_linear_fp8_exact_sums; partial sums are
+    multiples of 2^-6 below 2^13), in fp32 as they are, in bf16 rounded once."""
+    from hv_amd import ops
+    g = torch.Generator().manual_seed(k + m)
+
+    def codes(rows):
+        return (1 + torch.randint(0, 8, (rows, k), generator=g) / 8) * (torch.randint(0, 3, (rows, k), generator=g) - 1)
+
+    a, w = codes(m), codes(n)
+    f8 = torch.float8_e4m3fn
+    args = (a.to(f8).to(gpu_device), torch.ones(m, device=gpu_device), w.to(f8).to(gpu_device), torch.ones(n, device=gpu_device))
+    want = (a.double() @ w.double().t()).float()
+    for dtype in (F32, BF):
+        names = kernels_of(lambda: ops.linear_fp8(*args, out_dtype=dtype), "k_linear_fp8")
+        assert len(names) == 1 and tile in names.pop(), (names, tile)
+        assert torch.equal(ops.linear_fp8(*args, out_dtype=dtype).cpu(), want.to(dtype))
+    # scales, bias and activation on the last rows and columns, whose tiles are cut
+    sa, sw, b = (torch.rand(x, generator=g).to(gpu_device) + 0.5 for x in (m, n, n))
+    got = ops.linear_fp8(args[0], sa / 64, args[2], sw, bias=b, act="silu", out_dtype=F32)[-70:, -70:]
+    pre = want[-70:, -70:].double() * (sa[-70:, None] / 64).double().cpu() * sw[-70:].double().cpu() + b[-70:].double().cpu()
+    val = ACTS["silu"](pre)
+    # scale product, bias addition (2 e of each), slope 1.1 and evaluation 2^-20 as in test_linear_fp8
+    err = 1.13 * 4 * E * (pre.abs() + b[-70:].double().cpu()) + 2.0 ** -20 * (1 + pre.abs())
+    check(got, val, err + E * (val.abs() + err), "silu")
+
+
+@pytest.mark.parametrize("dtype,hq,hkv,d", [(BF, 32, 8, 128), (BF, 32, 4, 64), (BF, 64, 64, 32), (F32, 32, 8, 128), (F32, 32, 32, 64),
+                                            (F32, 32, 4, 32)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_packed_attention_many_rows(gpu_device, dtype, hq, hkv, d, causal):
+    """Rows enough for a wave per 32 of them in every type and tile width (rows * heads >= 2^16), several key tiles each:
+    forward and dQ without shared keys, and what dK / dV do there."""
+    from hv_amd import train_fn
+    lq, lk = [520, 300, 3, 611, 130, 484], [700, 300, 64, 611, 0, 300]
+    q, k, v, do, cq, ck = packed_inputs(lq, lk, hq, hkv, d, dtype, 27)
+    assert q.shape[0] * hq >= 1 << 16
+    x = [t.requires_grad_(True) for t in (q, k, v)]
+    out = train_fn.attention_packed(*x, cq, ck, causal=causal)
+    names = kernels_of(lambda: torch.autograd.grad(train_fn.attention_packed(*x, cq, ck, causal=causal), x, do),
+                       "k_attn_packed<", "k_attn_packed_dq<")
+    assert len(names) == 2 and all(", 1>" in n for n in names), names
+    val, tol = reference(q, k, v, cq, ck, causal, d ** -0.5, do)
+    for n, t in zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, x, do))):
+        check(t, val[n], tol[n], n)
+
+
+@pytest.mark.parametrize("f", [20.0, 60.0])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_packed_attention_gradients_of_large_scores(gpu_device, f, dtype):
+    """Scores of some thousands: weights are formed again from the log-sum-exp.  `off` in reference() grows with the scores
+    and is below 0.5 here, so that 4 off still bounds exp(2 off) - 1."""
+    from hv_amd import train_fn
+    q, k, v, do, cq, ck = packed_inputs([150, 33], [150, 70], 4, 2, 64, dtype, 28)
+    x = [t.requires_grad_(True) for t in (q.detach() * f, k.detach() * f, v)]
+    out = train_fn.attention_packed(*x, cq, ck, causal=True)
+    val, tol = reference(*x, cq, ck, True, 64 ** -0.5, do)
+    for n, t in zip(("out", "dq", "dk", "dv"), (out, *torch.autograd.grad(out, x, do))):
+        assert torch.isfinite(t).all()
+        check(t, val[n], tol[n], n)
+
+
+def test_packed_attention_few_rows_in_a_bounded_workspace(gpu_device):
+    """Many streams against histories: parts of the keys as short as for two blocks a CU would need over 256 MiB of partial
+    sums, so the parts are longer."""
+    import ctypes as C
+    from hv_amd import _lib, ops
+    lk = [1000 + 5 * (i % 13) for i in range(70)]
+    q, k, v, _, cq, ck = packed_inputs([1] * 70, lk, 32, 1, 128, BF, 29)
+    n = _lib.lib().hv_attn_packed_work_bytes(C.byref(ops.attn_packed_args(q, k, v, cq, ck, True, None)))
+    shortest = (-(-sum(lk) // 512) + 127) // 128 * 128
+    assert 0 < n <= 256 << 20 < -(-sum(lk) // shortest) * 70 * 32 * 132 * 4
+    out, lse = ops.attention_packed(q, k, v, cq, ck, causal=True, return_lse=True)
+    val, tol = reference(q, k, v, cq, ck, True, 128 ** -0.5)
+    check(out, val["out"], tol["out"], "out")
+    check(lse, val["lse"], tol["lse"], "lse")
