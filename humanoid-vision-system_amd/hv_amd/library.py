@@ -270,10 +270,10 @@ def _attn_packed_setup(ctx, inputs, output):
 
 
 def _attn_packed_bwd(ctx, do, dlse):
-    from .train_fn import PackedAttentionFn
+    from .train_fn import PackedAttentionLseFn
     q, k, v, cu_q, cu_k = ctx.saved_tensors
     causal, scale = ctx.meta
-    fn = lambda *x: PackedAttentionFn.apply(*(ops.dense_rows(t) for t in x), cu_q, cu_k, causal, scale)    # noqa: E731
+    fn = lambda *x: PackedAttentionLseFn.apply(*(ops.dense_rows(t) for t in x), cu_q, cu_k, causal, scale)    # noqa: E731
     g = _grad_of(fn, [q, k, v], [do, dlse])
     return g[0], g[1], g[2], None, None, None, None
 

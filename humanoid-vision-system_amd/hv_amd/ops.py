@@ -825,17 +825,21 @@ def _same_device(what: str, first: Tensor, *others) -> None:
 
 
 def row_strides(t: Tensor):
-    """(row, head) strides of `t` [rows, heads, d]; 0 where there is one row or one head, whose stride is never used."""
+    """(row, head) strides of `t` [rows, heads, d].  One off the 16-byte grid is 0 where there is one row or one head: it is
+    never used."""
     row, head, _ = t.stride()
-    return row if t.shape[0] > 1 else 0, head if t.shape[1] > 1 else 0
+    if (row | head) & 7:
+        return row if t.shape[0] > 1 else 0, head if t.shape[1] > 1 else 0
+    return row, head
 
 
 def rows_dense(t: Tensor) -> bool:
     """Whether attention_packed can read `t` [rows, heads, d] in place: last dimension dense, every row
     start on a 16-byte boundary."""
-    row, head = row_strides(t)
-    one = t.stride(2)
-    return (one == 1 or t.shape[2] == 1) and not (t.data_ptr() | row * t.element_size() | head * t.element_size()) & 15
+    row, head, one = t.stride()
+    if (row | head) & 7:
+        row, head = row_strides(t)
+    return (one == 1 or t.shape[2] == 1) and not (t.data_ptr() | (row | head) * t.element_size()) & 15
 
 
 def dense_rows(t: Tensor) -> Tensor:

@@ -518,11 +518,12 @@ def attention_packed_backward(q, k, v, cu_q, cu_k, call, out, low, lse, dout, ne
     # the kernels address 64 rows of q and dout with 32-bit offsets
     q, dout = (dense_rows(t) if max(row_strides(t)) < 1 << 22 else t.clone(memory_format=torch.contiguous_format)
                for t in (q, dout))
-    # as the forward had them, unless saved-tensor hooks returned them in another layout
-    k, v, lse = dense_rows(k), dense_rows(v), lse.contiguous()
-    out, low = (t if t is None or (t.is_contiguous() and not t.data_ptr() & 15)
-                else t.clone(memory_format=torch.contiguous_format) for t in (out, low))
     a = L.AttnPackedArgs.from_buffer_copy(call)
+    if (k.data_ptr() or None, v.data_ptr() or None, out.data_ptr() or None, lse.data_ptr() or None) != (a.k, a.v, a.out, a.lse):
+        # not the forward's tensors: saved-tensor hooks returned others, perhaps in another layout
+        k, v, lse = dense_rows(k), dense_rows(v), lse.contiguous()
+        out, low = (t if t is None or (t.is_contiguous() and not t.data_ptr() & 15)
+                    else t.clone(memory_format=torch.contiguous_format) for t in (out, low))
     attn_packed_point(a, q, k, v, cu_q, cu_k)
     dq = torch.empty(q.shape, device=q.device, dtype=q.dtype) if need_q else None
     dk = torch.empty(k.shape, device=q.device, dtype=q.dtype) if need_kv else None

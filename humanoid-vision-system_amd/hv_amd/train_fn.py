@@ -476,7 +476,7 @@ class AttentionFn(torch.autograd.Function):
 
 
 class PackedAttentionFn(torch.autograd.Function):
-    """Attention over packed sequences (ops.attention_packed) with its gradient: returns (out, lse)."""
+    """Attention over packed sequences (ops.attention_packed) with its gradient."""
 
     _hv_carries_state = True                             # reads no model options
 
@@ -484,20 +484,26 @@ class PackedAttentionFn(torch.autograd.Function):
     def forward(ctx, q, k, v, cu_q, cu_k, causal: bool, scale):
         out, low, lse, ctx.call = T.attention_packed_train(q, k, v, cu_q, cu_k, causal, scale)
         ctx.save_for_backward(q, k, v, cu_q, cu_k, out, low, lse)
-        ctx.set_materialize_grads(False)
-        return out, lse
+        return out
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, g, dlse):
+    def backward(ctx, g, dlse=None):
         q, k, v, cu_q, cu_k, out, low, lse = ctx.saved_tensors
-        if g is None:
-            if dlse is None:
-                return None, None, None, None, None, None, None
-            g = torch.zeros_like(out)
+        g = torch.zeros_like(out) if g is None else g    # only the log-sum-exp was used
         dq, dk, dv = T.attention_packed_backward(q, k, v, cu_q, cu_k, ctx.call, out, low, lse, g, _need(ctx, 0),
                                                  _need(ctx, 1) or _need(ctx, 2), dlse)
         return dq, dk, dv, None, None, None, None
+
+
+class PackedAttentionLseFn(PackedAttentionFn):
+    """PackedAttentionFn with the log-sum-exp as a second output: (out, lse), both differentiable."""
+
+    @staticmethod
+    def forward(ctx, *args):
+        out = PackedAttentionFn.forward(ctx, *args)
+        ctx.set_materialize_grads(False)
+        return out, ctx.to_save[-1]
 
 
 def attention_packed(q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Optional[Tensor] = None, *,
@@ -505,7 +511,7 @@ def attention_packed(q: Tensor, k: Tensor, v: Tensor, cu_q: Tensor, cu_k: Option
     """ops.attention_packed, differentiable in q, k and v.  Inputs that the kernels cannot read in place (last
     dimension not dense, rows not 16-byte aligned) are copied."""
     q, k, v = ops.dense_rows(q), ops.dense_rows(k), ops.dense_rows(v)
-    return PackedAttentionFn.apply(q, k, v, cu_q, cu_q if cu_k is None else cu_k, bool(causal), scale)[0]
+    return PackedAttentionFn.apply(q, k, v, cu_q, cu_q if cu_k is None else cu_k, bool(causal), scale)
 
 
 class AddRMSNormFn(torch.autograd.Function):
