@@ -810,7 +810,7 @@ int hv_quantize_rows_fp8(int dtype, const void* x, long ld, long rows, int cols,
    vit_encoder_decoder.py:146-152, on 8-bit rows); sums in fp32 (the 8-bit matrix instruction itself cuts the products
    of 8 consecutive k 13 binary places below their largest before it adds them); c fp32 or bf16.  k, lda and ldw are multiples
    of 16 and a, w 16-byte aligned; ceil(m / 256) * ceil(n / 256) up to 2^22, more is HV_EUNSUPPORTED.
-   work: hv_linear_fp8_work_bytes. */
+   work: hv_linear_fp8_work_bytes (0: no form needs any at present). */
 size_t hv_linear_fp8_work_bytes(long m, int n, int k);
 int hv_linear_fp8(const void* a, long lda, const float* a_scale, const void* w, long ldw, const float* w_scale,
                   const float* bias, int act, long m, int n, int k, int c_dtype, void* c, long ldc, void* work,
