@@ -6,7 +6,6 @@ import glob
 import os
 import re
 
-import pytest
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "humanoid-vision-system_amd", "csrc")
 
